@@ -33,12 +33,27 @@ EXPORTS = (
     "bc_merge_to_partial", "bc_tree_verify_commit", "bc_selftest_bounded_wait",
     "bc_cow_plan", "bc_tree_step", "bc_exchange_bytes", "bc_exchange_create",
     "bc_exchange_open", "bc_exchange_close", "bc_exchange_destroy", "bc_merge_exchange",
+    "bc_append_plan", "bc_append_kv", "bc_chunk_workspace_bytes", "bc_chunk_attention",
+    "bc_beam_workspace_bytes", "bc_beam_select", "bc_reorder_workspace_bytes",
+    "bc_beam_reorder",
 )
 
 
 class Shape(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in
                 ("batch", "query_heads", "kv_heads", "dim", "max_pages", "physical_pages")]
+
+
+class KvLayout(ctypes.Structure):
+    """Strides of a paged cache in elements (bc_kv_layout)."""
+    _fields_ = [(n, ctypes.c_longlong) for n in ("block_stride", "slot_stride", "head_stride")]
+
+
+class ChunkOptions(ctypes.Structure):
+    """Scores of a chunk attention (bc_chunk_options)."""
+    _fields_ = [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("window", ctypes.c_int),
+                ("alibi_slopes", ctypes.c_void_p), ("prefix", ctypes.c_void_p),
+                ("key_start", ctypes.c_void_p)]
 
 
 class BranchcraftError(RuntimeError):
@@ -51,6 +66,7 @@ _ll = ctypes.c_longlong
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
 _SP = ctypes.POINTER(Shape)
+_LP = ctypes.POINTER(KvLayout)
 
 _sigs = {
     "bc_decode": [_SP, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp],
@@ -81,6 +97,17 @@ _sigs = {
     "bc_exchange_close": [_vp],
     "bc_exchange_destroy": [_vp],
     "bc_merge_exchange": [_i, _i, ctypes.c_uint, _i, _i, _i, _vp, _vp, _vp, _vp, _vp],
+    "bc_append_plan": [_i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i,
+                       _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "bc_append_kv": [_SP, _i, _vp, _ll, _vp, _ll, _vp, _vp, _LP, _vp, _vp, _i, _vp, _vp],
+    "bc_chunk_workspace_bytes": [_SP, _i],
+    "bc_chunk_attention": [_SP, _i, _i, _vp, _ll, _vp, _vp, _LP, _vp, _vp, _vp,
+                           ctypes.POINTER(ChunkOptions), _vp, _i, _vp, _sz, _vp],
+    "bc_beam_workspace_bytes": [_i, _i, _i, _i],
+    "bc_beam_select": [_i, _i, _i, _i, _i, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
+    "bc_reorder_workspace_bytes": [_i, _i, _i],
+    "bc_beam_reorder": [_i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                        _vp, _sz, _vp],
     "bc_last_device_error": [_i],
     "bc_version": [],
 }
@@ -89,7 +116,9 @@ for _name, _args in _sigs.items():
     _fn.argtypes = _args
     _fn.restype = _i
 _lib.bc_last_device_error.restype = ctypes.c_uint
-_lib.bc_exchange_bytes.restype = _sz
+for _name in ("bc_exchange_bytes", "bc_chunk_workspace_bytes", "bc_beam_workspace_bytes",
+              "bc_reorder_workspace_bytes"):
+    getattr(_lib, _name).restype = _sz
 _lib.bc_version.restype = ctypes.c_char_p
 
 
@@ -345,3 +374,111 @@ def selftest_bounded_wait(ctas, smem_bytes, limit_us, stream=None):
 
 def last_device_error(reset: bool = True) -> int:
     return int(_lib.bc_last_device_error(1 if reset else 0))
+
+
+# ------------------------------------------------------------ prompts and beams
+
+DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def kv_layout(cache) -> KvLayout:
+    """The strides of a cache (or a view of one) shaped [P, 16, Hkv, D]."""
+    return KvLayout(cache.stride(0), cache.stride(1), cache.stride(2))
+
+
+class AppendPlan:
+    """Output buffers of bc_append_plan for `batch` sequences and at most
+    max_tokens new tokens."""
+
+    def __init__(self, batch, max_tokens, device="cuda"):
+        i32 = dict(dtype=torch.int32, device=device)
+        self.batch, self.max_tokens = batch, max_tokens
+        self.query_start = torch.empty(batch + 1, **i32)
+        self.slot_map = torch.empty(max_tokens, **i32)
+        self.positions = torch.empty(max_tokens, **i32)
+        self.clones = torch.empty(3, batch, **i32)
+        self.counts = torch.empty(3, **i32)
+        self.scratch = torch.empty(batch + 1, **i32)
+
+
+def append_plan(pages, lengths, new_tokens, state, plan: AppendPlan, state_out=None,
+                pages_out=None, lengths_out=None, stream=None):
+    """Plan new_tokens [batch] after lengths [batch]; state = (refcount [P],
+    free_stack [P], free_count [1]). Tables, lengths and state are updated in
+    place unless other arrays are given for them."""
+    out = state_out if state_out is not None else state
+    po = pages_out if pages_out is not None else pages
+    lo = lengths_out if lengths_out is not None else lengths
+    _check(_lib.bc_append_plan(plan.batch, state[0].numel(), _ptr(pages), pages.shape[1],
+                               _ptr(lengths), _ptr(new_tokens), *(_ptr(t) for t in state),
+                               *(_ptr(t) for t in out), _ptr(po), po.shape[1], _ptr(lo),
+                               plan.max_tokens, _ptr(plan.query_start), _ptr(plan.slot_map),
+                               _ptr(plan.positions), _ptr(plan.clones), _ptr(plan.counts),
+                               _ptr(plan.scratch), _stream(stream)), "bc_append_plan")
+
+
+def append_kv(shape: Shape, k, v, cache_k, cache_v, slot_map, clones=None, counts=None,
+              stream=None):
+    """k, v [tokens, Hkv, D] into the cache rows slot_map names, and a plan's clones."""
+    layout = kv_layout(cache_k)
+    _check(_lib.bc_append_kv(ctypes.byref(shape), k.shape[0], _ptr(k), k.stride(0), _ptr(v),
+                             v.stride(0), _ptr(cache_k), _ptr(cache_v), ctypes.byref(layout),
+                             _ptr(slot_map), _ptr(clones),
+                             0 if clones is None else clones.shape[1],
+                             None if counts is None else ctypes.c_void_p(counts.data_ptr() + 4),
+                             _stream(stream)), "bc_append_kv")
+
+
+def chunk_workspace_bytes(shape: Shape, tokens: int) -> int:
+    return _lib.bc_chunk_workspace_bytes(ctypes.byref(shape), tokens)
+
+
+def chunk_attention(shape: Shape, q, cache_k, cache_v, pages, query_start, lengths, output,
+                    workspace=None, scale=None, softcap=0.0, window=0, alibi_slopes=None,
+                    prefix=None, key_start=None, stream=None, check=True):
+    """Attention of q [tokens, Hq, D] over the paged keys; output of q's type or FP32."""
+    def dev(t):
+        return None if t is None else t.data_ptr()
+
+    options = ChunkOptions(scale if scale is not None else shape.dim ** -0.5, softcap, window,
+                           dev(alibi_slopes), dev(prefix), dev(key_start))
+    layout = kv_layout(cache_k)
+    rc = _lib.bc_chunk_attention(ctypes.byref(shape), q.shape[0], DTYPES[q.dtype], _ptr(q),
+                                 q.stride(0), _ptr(cache_k), _ptr(cache_v), ctypes.byref(layout),
+                                 _ptr(pages), _ptr(query_start), _ptr(lengths),
+                                 ctypes.byref(options), _ptr(output),
+                                 int(output.dtype == torch.float32), _ptr(workspace),
+                                 0 if workspace is None else workspace.numel(), _stream(stream))
+    if check:
+        _check(rc, "bc_chunk_attention")
+    return rc
+
+
+def beam_workspace_bytes(batch, beams, vocab, k) -> int:
+    return _lib.bc_beam_workspace_bytes(batch, beams, vocab, k)
+
+
+def beam_select(logits, scores, k, out_scores, out_tokens, out_parents, workspace, stream=None):
+    """logits [batch, beams, vocab], scores [batch, beams]; outputs [batch, k]."""
+    batch, beams, vocab = logits.shape
+    _check(_lib.bc_beam_select(batch, beams, vocab, k, DTYPES[logits.dtype], _ptr(logits),
+                               logits.stride(1), _ptr(scores), _ptr(out_scores),
+                               _ptr(out_tokens), _ptr(out_parents), _ptr(workspace),
+                               workspace.numel(), _stream(stream)), "bc_beam_select")
+
+
+def reorder_workspace_bytes(batch, beams_in, max_pages) -> int:
+    return _lib.bc_reorder_workspace_bytes(batch, beams_in, max_pages)
+
+
+def beam_reorder(pages, lengths, parents, state, pages_out, lengths_out, workspace,
+                 state_out=None, stream=None):
+    """pages [batch, beams, max_pages] after parents [batch, beams_out]; state as in
+    append_plan, updated in place unless state_out is given."""
+    batch, beams, max_pages = pages.shape
+    out = state_out if state_out is not None else state
+    _check(_lib.bc_beam_reorder(batch, beams, parents.shape[1], state[0].numel(), _ptr(pages),
+                                max_pages, _ptr(lengths), _ptr(parents),
+                                *(_ptr(t) for t in state), *(_ptr(t) for t in out),
+                                _ptr(pages_out), _ptr(lengths_out), _ptr(workspace),
+                                workspace.numel(), _stream(stream)), "bc_beam_reorder")

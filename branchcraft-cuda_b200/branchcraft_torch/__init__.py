@@ -56,6 +56,66 @@ def _fake_commit_batch(cache_k, cache_v, draft_k, draft_v, clone_src, clone_dst,
     return None
 
 
+def _fake_plan_outputs(pages, max_tokens):
+    batch = pages.shape[0]
+    return (pages.new_empty(batch + 1), pages.new_empty(max_tokens), pages.new_empty(max_tokens),
+            pages.new_empty((3, batch)), pages.new_empty(3))
+
+
+@torch.library.register_fake("branchcraft::append_plan")
+def _fake_append_plan(pages, lengths, new_tokens, refcount, free_stack, free_count, max_tokens,
+                      max_pages=0):
+    return (pages.new_empty((pages.shape[0], max_pages or pages.shape[1])),
+            torch.empty_like(lengths), torch.empty_like(refcount), torch.empty_like(free_stack),
+            torch.empty_like(free_count), *_fake_plan_outputs(pages, max_tokens))
+
+
+@torch.library.register_fake("branchcraft::append_plan_")
+def _fake_append_plan_(pages, lengths, new_tokens, refcount, free_stack, free_count, max_tokens):
+    return _fake_plan_outputs(pages, max_tokens)
+
+
+@torch.library.register_fake("branchcraft::append_kv_")
+def _fake_append_kv(cache_k, cache_v, k, v, slot_map, clones=None, counts=None):
+    return None
+
+
+@torch.library.register_fake("branchcraft::chunk_attention")
+def _fake_chunk_attention(q, k, v, pages, query_start, lengths, scale=None, softcap=0.0, window=0,
+                          alibi_slopes=None, prefix=None, key_start=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.register_fake("branchcraft::chunk_attention_out")
+def _fake_chunk_attention_out(q, k, v, pages, query_start, lengths, output, scale=None,
+                              softcap=0.0, window=0, alibi_slopes=None, prefix=None,
+                              key_start=None):
+    return output
+
+
+@torch.library.register_fake("branchcraft::beam_select")
+def _fake_beam_select(logits, scores, k):
+    out = scores.new_empty((scores.shape[0], k))
+    return out, out.new_empty(out.shape, dtype=torch.int32), out.new_empty(out.shape,
+                                                                          dtype=torch.int32)
+
+
+def _fake_rows(pages, parents):
+    batch, beams = parents.shape
+    return pages.new_empty((batch, beams, pages.shape[2])), pages.new_empty((batch, beams))
+
+
+@torch.library.register_fake("branchcraft::beam_reorder")
+def _fake_beam_reorder(pages, lengths, parents, refcount, free_stack, free_count):
+    return (*_fake_rows(pages, parents), torch.empty_like(refcount), torch.empty_like(free_stack),
+            torch.empty_like(free_count))
+
+
+@torch.library.register_fake("branchcraft::beam_reorder_")
+def _fake_beam_reorder_(pages, lengths, parents, refcount, free_stack, free_count):
+    return _fake_rows(pages, parents)
+
+
 def tree_verify(q, prefix_k, prefix_v, pages, lengths, draft_k, draft_v, parent):
     """Return FP32 [batch, candidate, query head, dimension] outputs."""
     return torch.ops.branchcraft.tree_verify(
@@ -98,3 +158,68 @@ def commit_batch_(cache_k, cache_v, draft_k, draft_v, clone_src, clone_dst, entr
     return torch.ops.branchcraft.commit_batch_(
         cache_k, cache_v, draft_k, draft_v, clone_src, clone_dst, entry_request, entry_node,
         entry_page, entry_slot)
+
+
+def append_plan(pages, lengths, new_tokens, refcount, free_stack, free_count, max_tokens,
+                max_pages=0):
+    """Give every sequence's new tokens their pages and slots under the pool's rules (reference
+    counts, free stack, copy-on-write). Returns the new (pages [S, max_pages or as before],
+    lengths, refcount, free_stack, free_count) and (query_start [S + 1], slot_map [max_tokens],
+    positions [max_tokens], clones [3, S], counts [3]: tokens, clones, status). A nonzero status
+    (1 bad counts, 2 pool exhausted, 3 malformed tables) plans nothing."""
+    return torch.ops.branchcraft.append_plan(pages, lengths, new_tokens, refcount, free_stack,
+                                             free_count, max_tokens, max_pages)
+
+
+def append_plan_(pages, lengths, new_tokens, refcount, free_stack, free_count, max_tokens):
+    """append_plan updating tables, lengths and pool state in place; returns (query_start,
+    slot_map, positions, clones, counts)."""
+    return torch.ops.branchcraft.append_plan_(pages, lengths, new_tokens, refcount, free_stack,
+                                              free_count, max_tokens)
+
+
+def append_kv_(cache_k, cache_v, k, v, slot_map, clones=None, counts=None):
+    """Write k, v [tokens, Hkv, D] into the slots of a plan (-1: skipped), and copy its clones'
+    valid slots, in one launch. Caches [P, 16, Hkv, D], strided views included."""
+    return torch.ops.branchcraft.append_kv_(cache_k, cache_v, k, v, slot_map, clones, counts)
+
+
+def chunk_attention(q, k, v, pages, query_start, lengths, scale=None, softcap=0.0, window=0,
+                    alibi_slopes=None, prefix=None, key_start=None):
+    """Attention of new tokens q [tokens, Hq, D] (request b: rows query_start[b] ..
+    query_start[b + 1], the last of its lengths[b] keys) over the paged caches k, v
+    [P, 16, Hkv, D]. Causal; `prefix` [B] opens a request's leading keys to all its tokens,
+    `window` keeps the last keys, `key_start` [tokens] is a token's first key (packed documents);
+    `softcap` caps scores by a tanh, `alibi_slopes` [Hq] take slope * distance off. Output of q's
+    type; rows of tokens in no request are unspecified (chunk_attention_out leaves them)."""
+    return torch.ops.branchcraft.chunk_attention(q, k, v, pages, query_start, lengths, scale,
+                                                 softcap, window, alibi_slopes, prefix, key_start)
+
+
+def chunk_attention_out(q, k, v, pages, query_start, lengths, output, scale=None, softcap=0.0,
+                        window=0, alibi_slopes=None, prefix=None, key_start=None):
+    """chunk_attention into a preallocated output of q's type or FP32 (CUDA-graph safe)."""
+    return torch.ops.branchcraft.chunk_attention_out(
+        q, k, v, pages, query_start, lengths, output, scale, softcap, window, alibi_slopes,
+        prefix, key_start)
+
+
+def beam_select(logits, scores, k):
+    """The k best (beam, token) pairs of every request by scores + log_softmax(logits):
+    (scores [B, k] FP32, tokens [B, k], parents [B, k]), best first, ties to the lowest
+    beam * vocab + token. logits [B, beams, vocab], scores [B, beams] FP32."""
+    return torch.ops.branchcraft.beam_select(logits, scores, k)
+
+
+def beam_reorder(pages, lengths, parents, refcount, free_stack, free_count):
+    """Page tables [B, beams, max_pages] after parents [B, new beams] (-1 drops a row): returns
+    (pages, lengths, refcount, free_stack, free_count), every new row forked from its parent,
+    every old one released, unheld pages pushed on the free stack."""
+    return torch.ops.branchcraft.beam_reorder(pages, lengths, parents, refcount, free_stack,
+                                              free_count)
+
+
+def beam_reorder_(pages, lengths, parents, refcount, free_stack, free_count):
+    """beam_reorder updating the pool's state in place; returns (pages, lengths)."""
+    return torch.ops.branchcraft.beam_reorder_(pages, lengths, parents, refcount, free_stack,
+                                               free_count)

@@ -16,8 +16,12 @@
 #include <cstdint>
 #include <cstring>
 #include <mutex>
+#include <utility>
 
+#include "bc_append.cuh"
 #include "bc_attn.cuh"
+#include "bc_beam.cuh"
+#include "bc_chunk.cuh"
 #include "bc_commit.cuh"
 #include "bc_cow_plan.cuh"
 #include "bc_exchange.cuh"
@@ -25,6 +29,9 @@
 #include "branchcraft.h"
 
 static_assert(bc::kCowPlanMaxNodes == BC_MAX_NODES, "the planner's node cap is the API's");
+static_assert(bc::kAppendMaxBatch == BC_MAX_SEQUENCES && bc::kBeamMax == BC_MAX_BEAMS &&
+                  bc::kBeamMaxVocab == BC_MAX_BEAM_VOCAB,
+              "the kernels' limits are the API's");
 
 namespace bc {
 
@@ -1010,6 +1017,330 @@ int bc_decode_static_scratch(const bc_shape* s, const void* q, const void* k, co
                            1.0f / std::sqrt(float(s->dim)), splits,
                            splits > 1 ? kSplitGlobal : kSplitNone, false, partial_a, partial_ml,
                            false, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+// ---------------------------------------------------------------------------
+// Prompts and beams (bc_append.cuh, bc_chunk.cuh, bc_beam.cuh).
+// ---------------------------------------------------------------------------
+}  // extern "C"
+
+namespace {
+
+// One launch as a programmatic dependent of the kernel before it.
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kern)(P...), dim3 grid, int threads, size_t smem,
+                             cudaStream_t stream, A&&... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads), 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...);
+}
+
+// Raises a kernel's dynamic shared memory limit once per device.
+template <typename K>
+cudaError_t raise_smem(K kern, size_t bytes, std::atomic<uint64_t>& configured, int dev) {
+  if (configured.load(std::memory_order_relaxed) & (uint64_t(1) << dev)) return cudaSuccess;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  if (e == cudaSuccess) configured.fetch_or(uint64_t(1) << dev);
+  return e;
+}
+
+uintptr_t address_bits() { return 0; }
+template <typename T, typename... R>
+uintptr_t address_bits(const T* p, R... rest) {
+  return reinterpret_cast<uintptr_t>(p) | address_bits(rest...);
+}
+
+// A cache whose rows the kernels may copy in 16-byte pieces.
+bool layout_ok(const bc_kv_layout* l) {
+  return l && l->block_stride >= 0 && l->slot_stride > 0 && l->head_stride > 0 &&
+         ((l->block_stride | l->slot_stride | l->head_stride) & 7) == 0;
+}
+
+// Pages whose slots an int can number.
+bool pool_ok(int pages) { return pages >= 1 && pages <= 0x7fffffff / kPageSize; }
+
+template <typename T>
+cudaError_t launch_beam_chunks(const BeamSelectParams& p, int dev, cudaStream_t stream) {
+  static std::atomic<uint64_t> configured{0};
+  const auto smem = [](int k) { return size_t(k) * 4 * kBeamPerThread * 8; };
+  const cudaError_t e = raise_smem(beam_chunk_kernel<T>, smem(kBeamMaxK), configured, dev);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(beam_chunk_kernel<T>, dim3(unsigned(p.batch) * p.beams * p.chunks),
+                          kBeamThreads, smem(p.k), stream, p);
+}
+
+size_t beam_merge_smem(long long lists, int k) {
+  return size_t(lists) * 8 + size_t((lists + 1) / 2) * 8 + size_t(k) * k * 12;
+}
+
+bool beam_shape_ok(int batch, int beams, int vocab, int k) {
+  return batch >= 1 && beams >= 1 && beams <= kBeamMax && vocab >= 1 && vocab <= kBeamMaxVocab &&
+         k >= 1 && k <= kBeamMaxK && k <= (long long)beams * vocab &&
+         (long long)batch * beams * ((vocab + kBeamChunk - 1) / kBeamChunk) <= 0x7fffffff;
+}
+
+int beam_chunks(int vocab) { return (vocab + kBeamChunk - 1) / kBeamChunk; }
+
+bool reorder_shape_ok(int batch, int beams_in, int max_pages) {
+  return batch >= 1 && beams_in >= 1 && beams_in <= kBeamMax && max_pages >= 1 &&
+         max_pages <= 0x7fffffff / kPageSize &&
+         (long long)batch * beams_in * ((max_pages + 31) / 32) * 32 <= 0x7fffffff;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bc_append_plan(int batch, int physical_pages, const int* pages_in, int max_pages_in,
+                   const int* lengths_in, const int* new_tokens, const int* refcount_in,
+                   const int* free_stack_in, const int* free_count_in, int* refcount,
+                   int* free_stack, int* free_count, int* pages_out, int max_pages_out,
+                   int* lengths_out, int max_tokens, int* query_start, int* slot_map,
+                   int* positions, int* clones, int* counts, int* scratch, void* stream) {
+  if (batch < 1 || batch > BC_MAX_SEQUENCES || !pool_ok(physical_pages) || !pool_ok(max_pages_in) ||
+      !pool_ok(max_pages_out) || max_tokens < 0 || !pages_in || !lengths_in || !new_tokens ||
+      !refcount_in || !free_stack_in || !free_count_in || !refcount || !free_stack ||
+      !free_count || !pages_out || !lengths_out || !query_start || !clones || !counts ||
+      !scratch || (max_tokens > 0 && (!slot_map || !positions)) ||
+      (pages_out == pages_in && max_pages_out != max_pages_in))
+    return cudaErrorInvalidValue;
+  const int dev = current_device();
+  if (dev < 0) return cudaErrorInvalidDevice;
+  static std::atomic<uint64_t> configured{0};
+  cudaError_t e =
+      raise_smem(append_plan_kernel, append_plan_smem_bytes(BC_MAX_SEQUENCES), configured, dev);
+  if (e != cudaSuccess) return e;
+  const AppendPlanParams p{batch, physical_pages, max_pages_in, max_pages_out, max_tokens,
+                           pages_in, lengths_in, new_tokens, refcount_in, free_stack_in,
+                           free_count_in, refcount, free_stack, free_count, pages_out,
+                           lengths_out, query_start, slot_map, positions, clones, counts,
+                           scratch};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool copy = refcount != refcount_in || free_stack != free_stack_in;
+  const int copiers = copy ? std::min(64, (physical_pages + 4 * kPlanThreads - 1) / (4 * kPlanThreads)) : 0;
+  e = launch_dependent(append_plan_kernel, dim3(unsigned(1 + copiers)), kPlanThreads,
+                       append_plan_smem_bytes(batch), st, p);
+  if (e != cudaSuccess) return e;
+  const int rows = kExpandThreads / 32;
+  const int row_blocks = (batch + rows - 1) / rows;
+  const int token_blocks = (max_tokens + kExpandTokens - 1) / kExpandTokens;
+  return launch_dependent(append_expand_kernel, dim3(unsigned(row_blocks + token_blocks)),
+                          kExpandThreads, 0, st, p, row_blocks);
+}
+
+int bc_append_kv(const bc_shape* s, int tokens, const void* k, long long k_stride, const void* v,
+                 long long v_stride, void* cache_k, void* cache_v, const bc_kv_layout* layout,
+                 const int* slot_map, const int* clones, int max_clones, const int* counts,
+                 void* stream) {
+  if (!s || s->kv_heads < 1 || (s->dim != 64 && s->dim != 128) || !pool_ok(s->physical_pages) ||
+      tokens < 0 || !cache_k || !cache_v || !layout_ok(layout) || max_clones < 0 ||
+      (tokens > 0 && (!k || !v || !slot_map)) || (max_clones > 0 && (!clones || !counts)) ||
+      (address_bits(k, v, cache_k, cache_v) % 16) || ((k_stride | v_stride) & 7) ||
+      k_stride < 0 || v_stride < 0 || (long long)s->kv_heads * s->dim > 0x7fffff)
+    return cudaErrorInvalidValue;
+  const int dev = current_device();
+  if (dev < 0) return cudaErrorInvalidDevice;
+  unsigned* err = error_word(dev);
+  if (!err) return cudaErrorInvalidDevice;
+  if (tokens == 0 && max_clones == 0) return cudaSuccess;
+  AppendKvParams p = {};
+  p.tokens = tokens;
+  p.head_vecs = s->dim / 8;
+  p.row_vecs = s->kv_heads * p.head_vecs;
+  p.physical_pages = s->physical_pages;
+  p.max_clones = max_clones;
+  p.k = static_cast<const uint4*>(k);
+  p.v = static_cast<const uint4*>(v);
+  p.k_stride = k_stride / 8;
+  p.v_stride = v_stride / 8;
+  p.cache_k = static_cast<uint4*>(cache_k);
+  p.cache_v = static_cast<uint4*>(cache_v);
+  p.block_stride = layout->block_stride / 8;
+  p.slot_stride = layout->slot_stride / 8;
+  p.head_stride = layout->head_stride / 8;
+  p.slot_map = slot_map;
+  p.clones = clones;
+  p.counts = counts;
+  p.err = err;
+  const int per_block = std::max(1, 4 * kAppendThreads / p.row_vecs);
+  const int token_blocks = (tokens + per_block - 1) / per_block;
+  return launch_dependent(append_kv_kernel, dim3(unsigned(token_blocks + max_clones), 2),
+                          kAppendThreads, 0, static_cast<cudaStream_t>(stream), p, token_blocks,
+                          per_block);
+}
+
+size_t bc_chunk_workspace_bytes(const bc_shape* s, int tokens) {
+  (void)s;
+  (void)tokens;
+  return 0;
+}
+
+int bc_chunk_attention(const bc_shape* s, int tokens, int dtype, const void* q,
+                       long long q_stride, const void* k, const void* v,
+                       const bc_kv_layout* layout, const int* pages, const int* query_start,
+                       const int* lengths, const bc_chunk_options* options, void* output,
+                       int output_f32, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!basic_shape_ok(s) || !pool_ok(s->physical_pages) || !pool_ok(s->max_pages) || tokens < 0 ||
+      (dtype != BC_F16 && dtype != BC_BF16) || s->query_heads / s->kv_heads > 128 || !q || !k ||
+      !v || !layout_ok(layout) || layout->head_stride % 64 || !pages || !query_start || !lengths ||
+      !options || !output || (address_bits(q, k, v, output) % 16) || (q_stride & 7) ||
+      q_stride < 0 || !(options->scale > 0.f) || std::isinf(options->scale) ||
+      !(options->softcap >= 0.f) || std::isinf(options->softcap) || options->window < 0 ||
+      workspace_bytes < bc_chunk_workspace_bytes(s, tokens) ||
+      (bc_chunk_workspace_bytes(s, tokens) > 0 && (!workspace || address_bits(workspace) % 16)))
+    return cudaErrorInvalidValue;
+  const int dev = current_device();
+  if (dev < 0) return cudaErrorInvalidDevice;
+  unsigned* err = error_word(dev);
+  if (!err) return cudaErrorInvalidDevice;
+  if (tokens == 0) return cudaSuccess;
+  ChunkParams p = {};
+  p.batch = s->batch;
+  p.tokens = tokens;
+  p.hq = s->query_heads;
+  p.hkv = s->kv_heads;
+  p.group = s->query_heads / s->kv_heads;
+  p.max_pages = s->max_pages;
+  p.physical_pages = s->physical_pages;
+  p.window = options->window;
+  p.q = q;
+  p.q_stride = q_stride;
+  p.k = k;
+  p.v = v;
+  p.block_stride = layout->block_stride;
+  p.slot_stride = layout->slot_stride;
+  p.head_stride = layout->head_stride;
+  p.pages = pages;
+  p.query_start = query_start;
+  p.lengths = lengths;
+  p.prefix = options->prefix;
+  p.key_start = options->key_start;
+  p.slopes = options->alibi_slopes;
+  p.out = output;
+  p.out_f32 = output_f32;
+  p.scale = options->scale;
+  p.softcap = options->softcap;
+  p.err = err;
+  p.token = next_launch_token();
+  const dim3 grid(unsigned(((long long)tokens * p.hq + 3) / 4));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (s->dim == 64)
+    return dtype == BC_F16 ? launch_dependent(chunk_rows_kernel<64, __half>, grid, 128, 0, st, p)
+                           : launch_dependent(chunk_rows_kernel<64, __nv_bfloat16>, grid, 128, 0, st, p);
+  return dtype == BC_F16 ? launch_dependent(chunk_rows_kernel<128, __half>, grid, 128, 0, st, p)
+                         : launch_dependent(chunk_rows_kernel<128, __nv_bfloat16>, grid, 128, 0, st, p);
+}
+
+size_t bc_beam_workspace_bytes(int batch, int beams, int vocab, int k) {
+  if (!beam_shape_ok(batch, beams, vocab, k)) return 0;
+  // per chunk: k keys, its sum and its largest logit
+  return size_t(batch) * beams * beam_chunks(vocab) * (size_t(k) * 8 + 8 + 4);
+}
+
+int bc_beam_select(int batch, int beams, int vocab, int k, int dtype, const void* logits,
+                   long long row_stride, const float* scores, float* out_scores, int* out_tokens,
+                   int* out_parents, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!beam_shape_ok(batch, beams, vocab, k) ||
+      (dtype != BC_F16 && dtype != BC_BF16 && dtype != BC_F32) || !logits || row_stride < vocab ||
+      !scores || !out_scores || !out_tokens || !out_parents || !workspace ||
+      address_bits(workspace) % 16 ||
+      address_bits(logits) % (dtype == BC_F32 ? 4 : 2) ||
+      workspace_bytes < bc_beam_workspace_bytes(batch, beams, vocab, k))
+    return cudaErrorInvalidValue;
+  const int dev = current_device();
+  if (dev < 0) return cudaErrorInvalidDevice;
+  BeamSelectParams p = {};
+  p.batch = batch;
+  p.beams = beams;
+  p.vocab = vocab;
+  p.k = k;
+  p.chunks = beam_chunks(vocab);
+  p.logits = logits;
+  p.row_stride = row_stride;
+  p.scores = scores;
+  p.out_scores = out_scores;
+  p.out_tokens = out_tokens;
+  p.out_parents = out_parents;
+  const size_t lists = size_t(batch) * beams * p.chunks;
+  p.keys = static_cast<unsigned long long*>(workspace);
+  p.chunk_sum = reinterpret_cast<double*>(p.keys + lists * k);
+  p.chunk_max = reinterpret_cast<float*>(p.chunk_sum + lists);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = dtype == BC_F16    ? launch_beam_chunks<__half>(p, dev, st)
+                  : dtype == BC_BF16 ? launch_beam_chunks<__nv_bfloat16>(p, dev, st)
+                                     : launch_beam_chunks<float>(p, dev, st);
+  if (e != cudaSuccess) return e;
+  static std::atomic<uint64_t> configured{0};
+  e = raise_smem(beam_merge_kernel,
+                 beam_merge_smem((long long)kBeamMax * beam_chunks(kBeamMaxVocab), kBeamMaxK),
+                 configured, dev);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(beam_merge_kernel, dim3(unsigned(batch)), kBeamThreads,
+                          beam_merge_smem((long long)beams * p.chunks, k), st, p);
+}
+
+size_t bc_reorder_workspace_bytes(int batch, int beams_in, int max_pages) {
+  if (!reorder_shape_ok(batch, beams_in, max_pages)) return 0;
+  return size_t(batch) * beams_in * ((max_pages + 31) / 32 + 1) * 4;
+}
+
+int bc_beam_reorder(int batch, int beams_in, int beams_out, int physical_pages,
+                    const int* pages_in, int max_pages, const int* lengths_in,
+                    const int* parents, const int* refcount_in, const int* free_stack_in,
+                    const int* free_count_in, int* refcount, int* free_stack, int* free_count,
+                    int* pages_out, int* lengths_out, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  if (!reorder_shape_ok(batch, beams_in, max_pages) || beams_out < 1 || beams_out > kBeamMax ||
+      !pool_ok(physical_pages) || !pages_in || !lengths_in || !parents || !refcount_in ||
+      !free_stack_in || !free_count_in || !refcount || !free_stack || !free_count || !pages_out ||
+      !lengths_out || pages_out == pages_in || lengths_out == lengths_in || !workspace ||
+      address_bits(workspace) % 4 ||
+      workspace_bytes < bc_reorder_workspace_bytes(batch, beams_in, max_pages))
+    return cudaErrorInvalidValue;
+  const int dev = current_device();
+  if (dev < 0) return cudaErrorInvalidDevice;
+  unsigned* err = error_word(dev);
+  if (!err) return cudaErrorInvalidDevice;
+  BeamReorderParams p = {};
+  p.batch = batch;
+  p.beams_in = beams_in;
+  p.beams_out = beams_out;
+  p.max_pages = max_pages;
+  p.physical_pages = physical_pages;
+  p.words = (max_pages + 31) / 32;
+  p.parents = parents;
+  p.pages_in = pages_in;
+  p.lengths_in = lengths_in;
+  p.refcount_in = refcount_in;
+  p.free_stack_in = free_stack_in;
+  p.free_count_in = free_count_in;
+  p.refcount = refcount;
+  p.free_stack = free_stack;
+  p.free_count = free_count;
+  p.pages_out = pages_out;
+  p.lengths_out = lengths_out;
+  p.marks = static_cast<unsigned*>(workspace);
+  p.children = static_cast<int*>(workspace) + size_t(batch) * beams_in * p.words;
+  p.err = err;
+  const int warps = kReorderThreads / 32;
+  const int row_blocks = int(((long long)batch * p.words + warps - 1) / warps);
+  const bool copy = refcount != refcount_in || free_stack != free_stack_in;
+  const int copiers =
+      copy ? std::min(64, (physical_pages + 4 * kReorderThreads - 1) / (4 * kReorderThreads)) : 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = launch_dependent(beam_rows_kernel, dim3(unsigned(row_blocks + copiers)),
+                                         kReorderThreads, 0, st, p, row_blocks);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(beam_release_kernel, dim3(1), kReleaseThreads, 0, st, p);
 }
 
 int bc_selftest_bounded_wait(int ctas, int smem_bytes, unsigned limit_us, void* stream) {

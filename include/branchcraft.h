@@ -314,6 +314,143 @@ int bc_decode_static_scratch(const bc_shape* shape, const void* q, const void* k
                              const void* v, const int* pages, const int* lengths,
                              float* output, int splits, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Prompts and beams: bring new tokens into the paged cache, attend with many of
+ * them at once, and search with beams over the copy-on-write page pool. None of
+ * this is in the reference. The 16-bit types are IEEE binary16 and bfloat16. */
+#define BC_F16 0
+#define BC_BF16 1
+#define BC_F32 2
+
+/* Where a cache row lies: element (page, slot, head, d) of K or V is at
+ * page*block_stride + slot*slot_stride + head*head_stride + d elements. The
+ * plain cache [P, 16, Hkv, D] has (16*Hkv*D, Hkv*D, D); vLLM's
+ * [P, 2, 16, Hkv, D] has (32*Hkv*D, Hkv*D, D) with V 16*Hkv*D elements on. */
+typedef struct bc_kv_layout {
+  long long block_stride;
+  long long slot_stride;
+  long long head_stride;
+} bc_kv_layout;
+
+/* Page tables, slot map and positions of new tokens, from the sequences'
+ * lengths and counts, under the page pool's rules (reference counts, free
+ * stack, copy-on-write of a shared partial last page), sequence b taking
+ * new_tokens[b] >= 0 tokens after its lengths_in[b], in batch order.
+ * State and tables are read from the *_in arrays and written to the others;
+ * each output may be its input (an update in place; pages_out only at equal
+ * width). Written:
+ *   pages_out [batch, max_pages_out] (-1 past a row's end, but for an update in
+ *     place, which writes only what changes), lengths_out [batch];
+ *   refcount [P], free_stack [P], free_count [1] (entries of the stack at or
+ *     past the count are left as they were);
+ *   query_start [batch + 1]: prefix sums of the counts; slot_map [max_tokens]:
+ *     page*16 + slot of every new token, sequence by sequence, and positions
+ *     [max_tokens], both -1 past the last token;
+ *   clones [3, batch]: source page, destination page and number of slots to
+ *     copy of every cloned page, -1 past the last;
+ *   counts [3]: tokens, clones, status. Status 0: planned; 1: a count below
+ *     zero, or more than max_tokens tokens; 2: not enough free pages; 3: a
+ *     length, page id, reference count or stack out of range, a row wider than
+ *     max_pages_out, more writers of a page than references to it, or holders
+ *     of one partial page at different lengths. On a nonzero status the state,
+ *     rows and lengths stay as they were and there are no tokens and no clones.
+ * scratch: batch + 1 ints. batch at most BC_MAX_SEQUENCES; the sequences of the
+ * batch are distinct (a row may hold pages of another, not be another). Two
+ * launches. */
+#define BC_MAX_SEQUENCES 4096
+int bc_append_plan(int batch, int physical_pages, const int* pages_in, int max_pages_in,
+                   const int* lengths_in, const int* new_tokens, const int* refcount_in,
+                   const int* free_stack_in, const int* free_count_in, int* refcount,
+                   int* free_stack, int* free_count, int* pages_out, int max_pages_out,
+                   int* lengths_out, int max_tokens, int* query_start, int* slot_map,
+                   int* positions, int* clones, int* counts, int* scratch, void* stream);
+
+/* New K/V rows into the cache: cache[slot_map[t]] = new[t] for t < tokens, and
+ * the page clones of a plan (clones [3, max_clones], counts [1] of them on the
+ * device as bc_append_plan writes them; both NULL for none) in the same launch.
+ * 16-bit elements of any kind. k and v are [tokens, Hkv, dim] with the given
+ * strides between tokens (parts of a fused projection, for instance). A slot of
+ * -1 is skipped; other slots outside [0, 16*P) and bad clones are skipped and
+ * set BC_ERR_COMMIT_INDEX. Slots are distinct: with a repeated one, which row's
+ * pieces stay is not defined. shape: kv_heads, dim and physical_pages are used.
+ * All addresses and strides are multiples of 16 bytes. */
+int bc_append_kv(const bc_shape* shape, int tokens, const void* k, long long k_stride,
+                 const void* v, long long v_stride, void* cache_k, void* cache_v,
+                 const bc_kv_layout* layout, const int* slot_map, const int* clones,
+                 int max_clones, const int* counts, void* stream);
+
+/* Scores of bc_chunk_attention. */
+typedef struct bc_chunk_options {
+  float scale;               /* > 0 */
+  float softcap;             /* 0: none; else scores become softcap*tanh(x/softcap) */
+  int window;                /* 0: none; else a token sees its last `window` keys, itself included */
+  const float* alibi_slopes; /* [query_heads] or NULL: x -= slope*|position - key| */
+  const int* prefix;         /* [batch] or NULL: keys below it are seen by every token of the request */
+  const int* key_start;      /* [tokens] or NULL: the first key a token sees (packed documents) */
+} bc_chunk_options;
+
+/* Attention of the new tokens of every request over its paged keys, which hold
+ * the new tokens' own rows already (bc_append_kv). Request b's tokens are rows
+ * query_start[b] .. query_start[b+1] of q [tokens, query_heads, dim] (q_stride
+ * elements between tokens) and the last ones of its lengths[b] keys; the token
+ * at position p sees the keys j with lo <= j < hi, hi = max(p + 1, prefix[b])
+ * (at most lengths[b]), lo = max(0, p + 1 - window, key_start[t]). A token
+ * without a key gets zeros. One token per request is a decode step. dtype
+ * (BC_F16 or BC_BF16) is that of q, k, v and, unless output_f32 != 0, of output
+ * [tokens, query_heads, dim], contiguous; rows in no request are left as they
+ * are. Sums are held in FP32; probabilities are rounded to dtype before the
+ * product with V. Slots past a request's length and pages that none of its
+ * tokens sees may hold anything; the values (V) of keys that some token of the
+ * request sees must be finite. Malformed starts and lengths are brought into
+ * range and set BC_ERR_LENGTH; a seen page outside the pool reads as zeros and
+ * sets BC_ERR_PAGE_RANGE. query_heads / kv_heads at most 128; addresses and
+ * strides are multiples of 16 bytes, head_stride one of 64 elements.
+ * workspace: bc_chunk_workspace_bytes, 16-byte aligned, one per call in
+ * flight (0 bytes: may be NULL). */
+size_t bc_chunk_workspace_bytes(const bc_shape* shape, int tokens);
+int bc_chunk_attention(const bc_shape* shape, int tokens, int dtype, const void* q,
+                       long long q_stride, const void* k, const void* v,
+                       const bc_kv_layout* layout, const int* pages, const int* query_start,
+                       const int* lengths, const bc_chunk_options* options, void* output,
+                       int output_f32, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The k best continuations of every request's beams: over (beam w, token v),
+ * scores[b, w] + logits[b, w, v] - log(sum_u exp logits[b, w, u]), the largest
+ * first, equal ones by the lowest w*vocab + v. logits [batch*beams, vocab] of
+ * `dtype` (BC_F16, BC_BF16, BC_F32), row_stride elements between rows; scores
+ * [batch, beams] FP32. A NaN logit counts as -inf and +inf as the largest
+ * number; a beam whose score is -inf or NaN, or all of whose logits are -inf,
+ * gives -inf. Written, [batch, k]: out_scores FP32, out_tokens, out_parents (the
+ * beam). 1 <= k <= min(64, beams*vocab), beams at most 64, vocab at most 2^20.
+ * workspace: bc_beam_workspace_bytes, 16-byte aligned, one per call in flight. */
+#define BC_MAX_BEAMS 64
+#define BC_MAX_BEAM_VOCAB (1 << 20)
+size_t bc_beam_workspace_bytes(int batch, int beams, int vocab, int k);
+int bc_beam_select(int batch, int beams, int vocab, int k, int dtype, const void* logits,
+                   long long row_stride, const float* scores, float* out_scores,
+                   int* out_tokens, int* out_parents, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/* The page tables after a beam step: row j of request b becomes that of beam
+ * parents[b, j] of the same request (-1: an empty row, the beam is dropped; out
+ * of range: as -1, and BC_ERR_PARENT). Reference counts change as if every new
+ * row were forked first and every old one released then, rows in order: pages
+ * nobody holds any more are pushed on the free stack in the order of their last
+ * release. pages_in [batch, beams_in, max_pages] and lengths_in are the old
+ * rows, pages_out [batch, beams_out, max_pages] (-1 past a row's end) and
+ * lengths_out [batch, beams_out] the new ones, in other memory; each array of
+ * the state may be its own input (an update in place). beams_in, beams_out at
+ * most BC_MAX_BEAMS; no request's pages are held at two columns. Page ids
+ * outside [0, P) set BC_ERR_PAGE_RANGE and are not counted. workspace:
+ * bc_reorder_workspace_bytes, one per call in flight. Two launches. */
+size_t bc_reorder_workspace_bytes(int batch, int beams_in, int max_pages);
+int bc_beam_reorder(int batch, int beams_in, int beams_out, int physical_pages,
+                    const int* pages_in, int max_pages, const int* lengths_in,
+                    const int* parents, const int* refcount_in, const int* free_stack_in,
+                    const int* free_count_in, int* refcount, int* free_stack, int* free_count,
+                    int* pages_out, int* lengths_out, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
 /* Self-test of the bounded waits every kernel here uses: `ctas` CTAs (with
  * smem_bytes of dynamic shared memory each, up to 200 KB, which sets how many
  * share an SM and so how many waves run) each wait on a barrier nothing
