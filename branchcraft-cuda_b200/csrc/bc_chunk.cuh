@@ -1,27 +1,58 @@
-// Attention of a chunk of new tokens over the paged cache: query row (token t
-// of request b, head h) at position p = length_b - n_b + i (i: the token's
-// place among the request's n_b) sees the keys lo <= j < hi,
+// Attention of a chunk of new tokens over the paged cache, on the 5th-generation
+// tensor cores. Query row (token t of request b, head h) at position
+// p = length_b - n_b + i (i: the token's place among the request's n_b) sees the
+// keys lo <= j < hi,
 //   hi = max(p + 1, prefix_b), lo = max(0, p + 1 - window, key_start_t),
 // with scores x_j = scale q.k_j, capped to softcap tanh(x_j / softcap), less
 // slope_h |p - j|; the output is sum_j exp(x_j - m) v_j / sum_j exp(x_j - m),
 // zeros where no key is seen.
+//
+// Work. A row tile is up to 128 (token, query head of one KV head) pairs, so a
+// K/V tile read once serves the whole group; an item is one block of two row
+// tiles of one request and KV head against the keys its rows see, in tiles of
+// 128 keys. Blocks with more than 128 rows are DUAL: softmax group g owns row
+// tile g and every key tile serves both. Smaller ones (a decode step: the group's
+// heads of one token) are ALT: both groups have the same rows and take alternate
+// key tiles, merged at the item's end.
+//
+// Schedule. One block per SM; the key tiles of all items, laid end to end, are
+// cut into equal shares, computed from the lengths on the device by every block
+// alike (no host round trip, no counters). A cut inside an item leaves FP32
+// partial states (m, l, O) that chunk_merge_kernel joins in order, so results do
+// not depend on timing.
+//
+// Warps: 0-3 and 4-7 softmax groups 0 and 1 (thread = row = TMEM lane), 8 the
+// scheduler (item descriptors, Q), 9 the MMA issuer, 10 and 11 the K/V producers
+// (alternate tiles of one ring, eight 16-row boxes each). TMEM: S of group g at
+// 128 g (P over its own S in 16-bit pairs), O of group g at 256 + 128 g.
 #pragma once
 
 #include <cuda_bf16.h>
+
+#include <type_traits>
 
 #include "bc_attn.cuh"
 
 namespace bc {
 
+constexpr int kChThreads = 384;
+constexpr int kChTile = 128;      // keys of a tile: eight pages
+constexpr int kChDescs = 4;       // item descriptors in flight
+constexpr int kChMaxBatch = 16384;
+constexpr int kChMinPiece = 4;    // key tiles: the granularity of cuts inside an item
+// Registers: launched at 168 a thread (65,536 / 384, in eights); the softmax
+// groups grow to 208 (a row's 128 scores stay in registers), the others shrink
+// to 88: together the launch's total.
+constexpr int kChLaunchRegs = 168, kChSoftmaxRegs = 208, kChOtherRegs = 88;
+static_assert(256 * kChSoftmaxRegs + 128 * kChOtherRegs == kChThreads * kChLaunchRegs,
+              "the register split must use exactly the launch budget");
+
 struct ChunkParams {
   int batch, tokens, hq, hkv, group;
+  int tile_tokens;            // tokens of a row tile: 128 / group
   int max_pages, physical_pages;
   int window;                 // 0: none
-  const void* q;
-  long long q_stride;         // elements between two tokens' rows
-  const void* k;
-  const void* v;
-  long long block_stride, slot_stride, head_stride;  // elements
+  int head_blocks;            // head stride in 64-element blocks
   const int* pages;           // [batch, max_pages]
   const int* query_start;     // [batch + 1]
   const int* lengths;         // [batch]
@@ -30,98 +61,923 @@ struct ChunkParams {
   const float* slopes;        // [hq] or null
   void* out;                  // [tokens, hq, D]
   int out_f32;
-  float scale, softcap;       // softcap 0: none
+  float scale_log2;           // scale * log2(e)
+  float cap_log2, cap_arg;    // softcap * log2(e), 2 log2(e) scale / softcap
+  // workspace of split items (null when none can be split)
+  float4* part_o;             // [blocks * 2][D / 4][part_rows]
+  float2* part_ml;            // [blocks * 2][part_rows]
+  int* sched;                 // [blocks][8]
+  int part_rows;
+  unsigned smem_bytes;        // dynamic shared memory of the launch
   unsigned* err;
   unsigned token;
 };
 
 // A request's rows and keys, with malformed values brought into range.
 struct ChunkRequest {
-  int first, n, len;  // first token, tokens, keys
+  int first, n, len, prefix;  // first token, tokens, keys, keys open to all
 };
 __device__ __forceinline__ ChunkRequest chunk_request(const ChunkParams& p, int b) {
   const int a = p.query_start[b], e = p.query_start[b + 1], len = p.lengths[b];
+  const int pre = p.prefix ? p.prefix[b] : 0;
   ChunkRequest r;
   r.first = min(max(a, 0), p.tokens);
   r.n = max(min(e, p.tokens) - r.first, 0);
   r.len = min(max(len, 0), p.max_pages * kPageSize);
+  r.prefix = min(max(pre, 0), r.len);
   if (a != r.first || e != r.first + r.n || len != r.len || r.len < r.n) atomicOr(p.err, kErrLength);
   return r;
 }
 
-// A warp per query row: every lane takes a key at a time, then a share of the
-// output's dimensions.
+// The keys that some row of a block of `cnt` tokens from the request's token
+// `i0` on may see, and their tiles (at least one: a block without keys still
+// writes its zeros).
+struct ChunkRange {
+  int lo, hi, t0, tiles;
+};
+__device__ __forceinline__ ChunkRange chunk_range(const ChunkParams& p, const ChunkRequest& r,
+                                                  int i0, int cnt) {
+  const int pos = r.len - r.n + i0;
+  ChunkRange g;
+  g.hi = max(max(pos + cnt, r.prefix), 0);
+  g.lo = p.window ? int(max((long long)pos + 1 - p.window, 0ll)) : 0;
+  if (p.key_start) {
+    int ks = 0x7fffffff;
+    for (int i = 0; i < cnt; ++i) ks = min(ks, p.key_start[r.first + i0 + i]);
+    g.lo = max(g.lo, ks);
+  }
+  g.lo = min(g.lo, g.hi);
+  g.t0 = g.lo / kChTile;
+  g.tiles = max((g.hi + kChTile - 1) / kChTile - g.t0, 1);
+  return g;
+}
+
+// One piece of an item, as every role reads it.
+struct ChunkDesc {
+  int first, ntok;       // the block's first token (row of q) and its tokens
+  int pos;               // position of the first
+  int prefix, lo, hi;    // keys open to all, and the block's range
+  int request, head;
+  int t0, nt;            // first key tile and number of tiles of this piece
+  int dual;              // two row tiles
+  int slot;              // partial state's place, or -1: the whole item
+  int end;               // no item: the last descriptor
+};
+
+template <int D>
+struct ChunkGeom {
+  static constexpr int KB = D / 64;
+  static constexpr int kRowTile = 128 * D * 2;   // Q of a row tile, K or V of a key tile
+  static constexpr int kPageBytes = 16 * D * 2;
+  static constexpr int kGroupBytes = KB * 1024;  // eight keys
+  static constexpr int kStages = D == 128 ? 5 : 8;
+  // barriers and small state lie before the 1024-byte aligned tiles
+  static constexpr int kBars = 2 * kStages + 2 + 10 + 2 * kChDescs + 1;
+  static constexpr int kMiscBytes = kBars * 8 + 16 + kChDescs * int(sizeof(ChunkDesc));
+  static constexpr int kQOff = 0;
+  static constexpr int kRingOff = 2 * kRowTile;
+  static constexpr int kMlOff = kRingOff + kStages * kRowTile;  // [2][128] (m, l)
+  static constexpr int kTileBytes = kMlOff + 2 * 128 * 8;
+  static_assert(kMiscBytes <= 1008, "the small state fits before the first tile");
+  static_assert(kChMaxBatch * 8 <= kStages * kRowTile, "the plan's sums fit in the ring");
+  // with `fixed` bytes of static shared memory before the dynamic part
+  static size_t smem_bytes(size_t fixed) {
+    const size_t at = (fixed + 15) / 16 * 16;
+    return (at + kMiscBytes + 1023) / 1024 * 1024 - at + kTileBytes;
+  }
+  static constexpr uint32_t kTmemO = 256, kTmemCols = 512;
+};
+
+// 5-D tiled load: one page's 16 rows of one head as [2][KB][8][128 bytes], so
+// that consecutive pages continue the same row of 8-key groups.
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2, int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2),
+      "r"(c3), "r"(c4)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+// Waits out copies in flight on a failing launch: as mbar_wait, but deaf to the
+// launch's abort mark (at most 10 ms).
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+  const unsigned long long start = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity) && globaltimer_ns() - start < 10000000ull) {
+  }
+}
+
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Two FP32 lanes in one instruction: (a0, a1) * (b, b) + (c, c).
+__device__ __forceinline__ void fma_pair(float a0, float a1, float b, float c, float& d0,
+                                         float& d1) {
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b), "f"(c));
+}
+__device__ __forceinline__ void add_pair(float& a0, float& a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b0), "f"(b1));
+}
+
+// The place of K or V tile j of an item of nt tiles in the ring's order: `lag`
+// K tiles first (one for DUAL items, whose first two products share it; two for
+// ALT), then V and K in turn, then the V tiles left over.
+__device__ __forceinline__ int chunk_kseq(int j, int lag) { return j < lag ? j : 2 * j - lag + 1; }
+__device__ __forceinline__ int chunk_vseq(int j, int lag, int nt) { return min(j + lag, nt) + j; }
+
+// MOD: bit 0 the tanh cap, bit 1 the distance bias.
+template <int D, typename T, int MOD>
+__global__ void __launch_bounds__(kChThreads, 1)
+    chunk_mma_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap qmap,
+                     const __grid_constant__ CUtensorMap kmap,
+                     const __grid_constant__ CUtensorMap vmap) {
+  using G = ChunkGeom<D>;
+  constexpr int KB = G::KB, NS = G::kStages;
+  constexpr float kNegInf = -INFINITY;
+  constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
+  constexpr uint32_t kIdescS = umma_idesc_f16(128, kChTile, false, false) | kBf16;
+  constexpr uint32_t kIdescPV = umma_idesc_f16(128, D, false, true) | kBf16;
+
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* tiles = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + G::kMiscBytes + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw);  // [NS] K or V tile landed
+  uint64_t* empty = full + NS;                             // [NS] its products are done
+  uint64_t* q_full = empty + NS;
+  uint64_t* q_free = q_full + 1;        // the item's S products are done
+  uint64_t* s_full = q_free + 1;        // [2] S of group g
+  uint64_t* p_full = s_full + 2;        // [2] P of group g written (4 warps)
+  uint64_t* o_full = p_full + 2;        // [2] the item's last product of group g
+  uint64_t* xch = o_full + 2;           // [2] ALT: group g's (m, l) written (4 warps)
+  uint64_t* xch_done = xch + 2;         // [2] ALT: group g has read both O (4 warps)
+  uint64_t* desc_full = xch_done + 2;   // [kChDescs]
+  uint64_t* desc_empty = desc_full + kChDescs;  // [kChDescs] read by 11 warps
+  uint64_t* fin = desc_empty + kChDescs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin + 1);
+  ChunkDesc* descs = reinterpret_cast<ChunkDesc*>(reinterpret_cast<uint8_t*>(fin + 1) + 16);
+  float2* ml_x = reinterpret_cast<float2*>(tiles + G::kMlOff);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (uint32_t(tiles - smem_raw) + G::kTileBytes > p.smem_bytes) {  // (never: the host's sum)
+    if (tid == 0) atomicOr(p.err, kErrTimeout);
+    return;
+  }
+  if (tid == 0) {
+    s_launch_token = p.token;
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_free, 1);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&s_full[g], 1);
+      mbar_init(&p_full[g], 4);
+      mbar_init(&o_full[g], 1);
+      mbar_init(&xch[g], 4);
+      mbar_init(&xch_done[g], 4);
+    }
+    for (int s = 0; s < kChDescs; ++s) {
+      mbar_init(&desc_full[s], 1);
+      mbar_init(&desc_empty[s], 11);
+    }
+    mbar_init(fin, 1);
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, G::kTmemCols);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  if (warp == 8 && lane < 3) prefetch_tmap(lane == 0 ? &qmap : lane == 1 ? &kmap : &vmap);
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tmem_slot;
+  grid_launch_dependents();  // (TMEM is allocated: a waiting successor cannot hold it back)
+  grid_dependency_wait();
+
+  // ---- plan: key tiles of every request (per KV head), into the idle ring
+  const int block_tokens = 2 * p.tile_tokens;
+  long long* tot = reinterpret_cast<long long*>(tiles + G::kRingOff);
+  for (int base = warp * 32; base < p.batch; base += (kChThreads / 32) * 32) {
+    const int b = base + lane;
+    ChunkRequest r = {0, 0, 0, 0};
+    if (b < p.batch) r = chunk_request(p, b);
+    const int nblk = (r.n + block_tokens - 1) / block_tokens;
+    long long sum = 0;
+    if (nblk <= 4)
+      for (int j = 0; j < nblk; ++j)
+        sum += chunk_range(p, r, j * block_tokens, min(block_tokens, r.n - j * block_tokens)).tiles;
+    for (unsigned many = __ballot_sync(0xffffffffu, nblk > 4); many; many &= many - 1) {
+      const int src = __ffs(many) - 1;  // a long chunk: its blocks spread over the warp
+      const ChunkRequest o = {__shfl_sync(0xffffffffu, r.first, src),
+                              __shfl_sync(0xffffffffu, r.n, src),
+                              __shfl_sync(0xffffffffu, r.len, src),
+                              __shfl_sync(0xffffffffu, r.prefix, src)};
+      long long part = 0;
+      for (int i0 = lane * block_tokens; i0 < o.n; i0 += 32 * block_tokens)
+        part += chunk_range(p, o, i0, min(block_tokens, o.n - i0)).tiles;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+      if (lane == src) sum = part;
+    }
+    if (b < p.batch) tot[b] = sum;
+  }
+  fence_proxy_async_smem();  // (copies will follow into the same memory)
+  __syncthreads();
+
+  const uint32_t lane_addr = uint32_t((warp & 3) * 32) << 16;
+  bool ok = true;
+  if (warp >= 8) {
+    regs_decrease<kChOtherRegs>();
+    if (warp == 8) {
+      // ---------------------------------------------------------- scheduler
+      const int per_lane = (p.batch + 31) / 32;
+      const int sb0 = min(p.batch, lane * per_lane), sb1 = min(p.batch, sb0 + per_lane);
+      long long mine = 0;
+      for (int b = sb0; b < sb1; ++b) mine += tot[b];
+      long long incl = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += up;
+      }
+      const long long per_head = __shfl_sync(0xffffffffu, incl, 31);
+      const long long units = per_head * p.hkv;
+      const long long pre = incl - mine;
+      // Cuts inside an item fall on multiples of `grain` tiles from its start
+      // (an eighth of a share, at least kChMinPiece: a piece costs its partial
+      // state's way through memory) or on its ends.
+      const long long share = units / gridDim.x;
+      const int grain = int(max((long long)kChMinPiece, min(share / 8, 1ll << 20)));
+      int req = 0, blk = 0, head = 0, off = 0, n_tiles = 1;
+      ChunkRequest r = {0, 0, 0, 0};
+      ChunkRange g = {0, 0, 0, 1};
+      auto cut = [&](long long u) -> long long {  // finds unit u and moves it to a cut
+        if (u <= 0 || u >= units) {
+          if (u >= units) return units;
+          u = 0;
+        }
+        const unsigned below = __ballot_sync(0xffffffffu, mine > 0 && pre * p.hkv <= u);
+        const int src = 31 - __clz(below);
+        int found = 0;
+        long long at = pre;
+        if (lane == src)
+          for (found = sb0; (at + tot[found]) * p.hkv <= u; ++found) at += tot[found];
+        req = __shfl_sync(0xffffffffu, found, src);
+        long long rem = u - __shfl_sync(0xffffffffu, at, src) * p.hkv;
+        r = chunk_request(p, req);
+        const int nblk = (r.n + block_tokens - 1) / block_tokens;
+        for (int j0 = 0;; j0 += 32) {  // the block among the request's
+          const int j = j0 + lane;
+          const int t = j < nblk ? chunk_range(p, r, j * block_tokens,
+                                               min(block_tokens, r.n - j * block_tokens)).tiles
+                                 : 0;
+          long long in = t;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const long long up = __shfl_up_sync(0xffffffffu, in, d);
+            if (lane >= d) in += up;
+          }
+          const unsigned after = __ballot_sync(0xffffffffu, in * p.hkv > rem);
+          if (after) {
+            const int w = __ffs(after) - 1;
+            blk = j0 + w;
+            n_tiles = __shfl_sync(0xffffffffu, t, w);
+            rem -= (__shfl_sync(0xffffffffu, in, w) - n_tiles) * p.hkv;
+            break;
+          }
+          rem -= __shfl_sync(0xffffffffu, in, 31) * p.hkv;
+        }
+        head = int(rem / n_tiles);
+        off = int(rem % n_tiles);
+        const int was = off;
+        off = (off + grain / 2) / grain * grain;
+        if (off > 0 && n_tiles - off < (grain + 1) / 2) off = n_tiles;
+        return u - was + off;
+      };
+      const long long u1 = cut(units * (blockIdx.x + 1) / gridDim.x);
+      const long long u0 = cut(units * blockIdx.x / gridDim.x);
+      long long left = u0 < units ? u1 - u0 : 0;
+      auto load_block = [&] {  // the current block's range
+        g = chunk_range(p, r, blk * block_tokens,
+                        min(block_tokens, r.n - blk * block_tokens));
+        n_tiles = g.tiles;
+      };
+      auto next_item = [&] {
+        off = 0;
+        if (++head < p.hkv) return;
+        head = 0;
+        if ((++blk) * block_tokens >= r.n) {
+          blk = 0;
+          // the next request with tokens (the sums of the plan are gone: the
+          // ring is in use), 32 looked at together
+          for (++req; req < p.batch; req += 32) {
+            const int b = req + lane;
+            const bool some = b < p.batch && chunk_request(p, b).n > 0;
+            const unsigned with = __ballot_sync(0xffffffffu, some);
+            if (with) {
+              req += __ffs(with) - 1;
+              break;
+            }
+          }
+          if (req < p.batch) r = chunk_request(p, req);
+        }
+        if (req < p.batch) load_block();
+      };
+      // for the merge: the first piece continues an item that goes on (1) or ends
+      // (2) here, or this block has no share (3); and the item that starts here
+      // and goes on
+      int cont = left > 0 ? 0 : 3, has = 0, h_first = 0, h_ntok = 0, h_head = 0;
+      if (left > 0) {
+        load_block();
+        if (off >= n_tiles) next_item();
+      }
+      int k = 0;
+      bool q_pending = false;
+      for (;; ++k) {
+        ChunkDesc d = {};
+        d.end = left <= 0;
+        if (!d.end) {
+          const int i0 = blk * block_tokens;
+          d.first = r.first + i0;
+          d.ntok = min(block_tokens, r.n - i0);
+          d.pos = r.len - r.n + i0;
+          d.prefix = r.prefix;
+          d.lo = g.lo;
+          d.hi = g.hi;
+          d.request = req;
+          d.head = head;
+          d.t0 = g.t0 + off;
+          d.nt = int(min((long long)(n_tiles - off), left));
+          d.dual = d.ntok > p.tile_tokens;
+          const bool whole = off == 0 && d.nt == n_tiles;
+          d.slot = whole ? -1 : int(blockIdx.x) * 2 + (off == 0 ? 1 : 0);
+          if (!whole && off == 0) {
+            has = 1;
+            h_first = d.first;
+            h_ntok = d.ntok;
+            h_head = head;
+          }
+          if (off > 0) cont = off + d.nt == n_tiles ? 2 : 1;
+        }
+        const int ds = k % kChDescs;
+        if (k >= kChDescs)
+          ok = __all_sync(0xffffffffu, mbar_wait(&desc_empty[ds], ((k / kChDescs) - 1) & 1));
+        if (!ok) break;
+        if (lane == 0) {
+          descs[ds] = d;
+          mbar_arrive(&desc_full[ds]);
+        }
+        __syncwarp();
+        if (d.end) break;
+        if (k > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_free, (k - 1) & 1));
+        if (!ok) break;
+        // Q of the block's row tiles; rows past the request's are other tokens'
+        // (or zeros past the last): computed, never stored.
+        const int nq = d.dual ? 2 : 1;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(q_full, uint32_t(nq * KB * p.tile_tokens * p.group * 128));
+          for (int i = 0; i < nq; ++i)
+            for (int kb = 0; kb < KB; ++kb)
+              tma_load_3d(tiles + G::kQOff + i * G::kRowTile + kb * (128 * 128), &qmap, q_full,
+                          kb * 64, d.head * p.group, d.first + i * p.tile_tokens);
+        }
+        __syncwarp();
+        q_pending = true;
+        left -= d.nt;
+        if (left > 0) next_item();
+      }
+      if (p.sched && lane == 0) {
+        int* s = p.sched + size_t(blockIdx.x) * 8;
+        s[0] = cont;
+        s[1] = has;
+        s[2] = h_first;
+        s[3] = h_ntok;
+        s[4] = h_head;
+      }
+      if (!ok && q_pending) mbar_drain(q_full, (k - (k > 0)) & 1);
+    } else if (warp == 9) {
+      // -------------------------------------------------------------- MMAs
+      const uint64_t qdesc = umma_desc_sw128(smem_u32(tiles + G::kQOff), 16, 1024);
+      const uint64_t kdesc0 = umma_desc_sw128(smem_u32(tiles + G::kRingOff), 16, G::kGroupBytes);
+      const uint64_t vdesc0 = umma_desc_sw128(smem_u32(tiles + G::kRingOff), 1024, G::kGroupBytes);
+      unsigned seq0 = 0;           // ring place of the item's first tile
+      uint32_t pc[2] = {0u, 0u};   // P tiles taken of each group
+      for (int k = 0; ok; ++k) {
+        const int ds = k % kChDescs;
+        ok = __all_sync(0xffffffffu, mbar_wait(&desc_full[ds], (k / kChDescs) & 1));
+        if (!ok) break;
+        const int nt = descs[ds].nt, dual = descs[ds].dual, end = descs[ds].end;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&desc_empty[ds]);
+        if (end) break;
+        const int lag = dual ? 1 : 2;
+        const int n_of[2] = {dual ? nt : (nt + 1) / 2, dual ? nt : nt / 2};
+        ok = __all_sync(0xffffffffu, mbar_wait(q_full, k & 1));
+        if (!ok) break;
+        for (int n = 0; n <= n_of[0] && ok; ++n) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (n > 0 && n - 1 < n_of[g] && ok) {  // O_g += P_g V
+              const int j = dual ? n - 1 : 2 * (n - 1) + g;
+              const unsigned s = seq0 + unsigned(chunk_vseq(j, lag, nt));
+              const int st = int(s % NS);
+              ok = __all_sync(0xffffffffu, mbar_wait(&p_full[g], pc[g] & 1) &&
+                                               mbar_wait(&full[st], (s / NS) & 1));
+              if (!ok) break;
+              ++pc[g];
+              tc_fence_after();
+              const uint64_t vd = vdesc0 + uint64_t((st * G::kRowTile) >> 4);
+#pragma unroll
+              for (int kk = 0; kk < kChTile / 16; ++kk)
+                if (elect_one())
+                  umma_f16_ts(tbase + G::kTmemO + g * 128, tbase + g * 128 + kk * 8,
+                              vd + uint64_t((kk * 2 * G::kGroupBytes) >> 4), kIdescPV,
+                              (n > 1 || kk > 0) ? 1u : 0u);
+              if (elect_one()) {
+                if (!dual || g == 1) umma_commit(&empty[st]);
+                if (n == n_of[g]) umma_commit(&o_full[g]);
+              }
+              __syncwarp();
+            }
+            if (n < n_of[g] && ok) {  // S_g = Q_g K^T (over the P just read)
+              const int j = dual ? n : 2 * n + g;
+              const unsigned s = seq0 + unsigned(chunk_kseq(j, lag));
+              const int st = int(s % NS);
+              ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (s / NS) & 1));
+              if (!ok) break;
+              tc_fence_after();
+              const uint64_t qd = qdesc + uint64_t((dual ? g * G::kRowTile : 0) >> 4);
+              const uint64_t kd = kdesc0 + uint64_t((st * G::kRowTile) >> 4);
+#pragma unroll
+              for (int ks = 0; ks < D / 16; ++ks)
+                if (elect_one())
+                  umma_f16(tbase + g * 128, qd + uint64_t(((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4),
+                           kd + uint64_t(((ks >> 2) * 1024 + (ks & 3) * 32) >> 4), kIdescS,
+                           ks > 0 ? 1u : 0u);
+              if (elect_one()) {
+                umma_commit(&s_full[g]);
+                if (!dual || g == 1) umma_commit(&empty[st]);
+                // the item's last S product: of group 1 when it has as many tiles
+                if (n == n_of[0] - 1 && (g == 1 || n_of[1] < n_of[0])) umma_commit(q_free);
+              }
+              __syncwarp();
+            }
+          }
+        }
+        // (an ALT item of one tile has no product of group 1)
+        if (ok && n_of[1] == 0) {
+          if (elect_one()) umma_commit(&o_full[1]);
+          __syncwarp();
+        }
+        seq0 += 2u * unsigned(nt);
+      }
+      if (elect_one()) umma_commit(fin);
+      __syncwarp();
+      if (lane == 0) mbar_drain(fin, 0);
+      __syncwarp();
+    } else {
+      // ---------------------------------------------------------- producers
+      // Ring places of parity `par`; lane l holds the page id of page (l & 7) of
+      // this warp's step 4 batch + l / 8, loaded a batch ahead.
+      const int par = warp - 10;
+      unsigned seq0 = 0, last = 0;
+      bool any = false;
+      for (int k = 0; ok; ++k) {
+        const int ds = k % kChDescs;
+        ok = __all_sync(0xffffffffu, mbar_wait(&desc_full[ds], (k / kChDescs) & 1));
+        if (!ok) break;
+        const ChunkDesc d = descs[ds];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&desc_empty[ds]);
+        if (d.end) break;
+        const int nt = d.nt, lag = min(d.dual ? 1 : 2, nt), steps = nt;  // of 2 nt places
+        const int* row = p.pages + size_t(d.request) * p.max_pages;
+        auto tile_of = [&](int s, bool& is_v) -> int {  // ring place -> tile
+          if (s < lag) {
+            is_v = false;
+            return s;
+          }
+          s -= lag;
+          if (s < 2 * (nt - lag)) {
+            is_v = (s & 1) == 0;
+            return is_v ? s >> 1 : (s >> 1) + lag;
+          }
+          is_v = true;
+          return s - (nt - lag);
+        };
+        auto load_id = [&](int first) -> int {
+          const int i = first + (lane >> 3);
+          if (i >= steps) return -1;
+          bool is_v;
+          const int pg = (d.t0 + tile_of(par + 2 * i, is_v)) * (kChTile / kPageSize) + (lane & 7);
+          // pages that no row of the block sees stay out: the copy fills zeros
+          if (pg * kPageSize >= d.hi || (pg + 1) * kPageSize <= d.lo) return -1;
+          const int id = __ldg(row + pg);
+          if (id < 0 || id >= p.physical_pages) {
+            atomicOr(p.err, kErrPageRange);
+            return -1;
+          }
+          return id;
+        };
+        int cur = load_id(0), nxt = load_id(4);
+        for (int i = 0; i < steps; ++i) {
+          if (i > 0 && (i & 3) == 0) {
+            cur = nxt;
+            nxt = load_id(i + 4);
+          }
+          const unsigned s = seq0 + unsigned(par + 2 * i);
+          const int st = int(s % NS);
+          if (s >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], ((s / NS) - 1) & 1));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&full[st], uint32_t(G::kRowTile));
+          const int id = __shfl_sync(0xffffffffu, cur, (i & 3) * 8 + (lane & 7));
+          bool is_v;
+          tile_of(par + 2 * i, is_v);
+          if (lane < 8)
+            tma_load_5d(tiles + G::kRingOff + st * G::kRowTile + lane * G::kPageBytes,
+                        is_v ? &vmap : &kmap, &full[st], 0, 0, d.head * p.head_blocks, 0, id);
+          __syncwarp();
+          last = s;
+          any = true;
+        }
+        seq0 += 2u * unsigned(nt);
+      }
+      if (!ok && any)  // this warp's copies in flight: its last places
+        for (unsigned s = last; last - s < NS; s -= 2) {
+          if (lane == 0) mbar_drain(&full[s % NS], (s / NS) & 1);
+          __syncwarp();
+          if (s < 2) break;
+        }
+    }
+    if (!ok && lane == 0) atomicOr(p.err, kErrTimeout);
+    tc_fence_before();
+    named_barrier_sync(1, kChThreads);  // every TMEM read and product is done
+    if (warp == 9) {
+      tc_fence_after();
+      tmem_dealloc(tbase, G::kTmemCols);
+    }
+    return;
+  }
+  // (the softmax path never rejoins the other: each keeps its register budget)
+  {
+    // --------------------------------------------------------------- softmax
+    regs_increase<kChSoftmaxRegs>();
+    const int grp = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t tS = tbase + lane_addr + uint32_t(grp) * 128;
+    const uint32_t tO = tbase + lane_addr + G::kTmemO + uint32_t(grp) * 128;
+    const int row_tok = row / p.group, row_head = row % p.group;
+    uint32_t sc = 0, alt = 0;  // S tiles taken; ALT items done
+    unsigned seq0 = 0;
+    for (int k = 0; ok; ++k) {
+      const int ds = k % kChDescs;
+      ok = __all_sync(0xffffffffu, mbar_wait(&desc_full[ds], (k / kChDescs) & 1));
+      if (!ok) break;
+      const ChunkDesc d = descs[ds];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&desc_empty[ds]);
+      if (d.end) break;
+      const bool dual = d.dual != 0;
+      const int lag = dual ? 1 : 2;
+      const int n_mine = dual ? d.nt : (d.nt + 1 - grp) / 2;
+      const int tok = (dual ? grp * p.tile_tokens : 0) + row_tok;
+      const bool valid = row_tok < p.tile_tokens && tok < d.ntok;
+      const int head = d.head * p.group + row_head;
+      const int pos = d.pos + tok;
+      // the row's keys (a row of nobody keeps all of them, so as not to send its
+      // warp down the masked path: its results are dropped)
+      int lo = 0, hi = 0x7fffffff;
+      if (valid) {
+        hi = max(pos + 1, d.prefix);
+        if (p.window) lo = int(max((long long)pos + 1 - p.window, 0ll));
+        if (p.key_start) lo = max(lo, __ldg(p.key_start + d.first + tok));
+      }
+      float slope = 0.f;
+      if ((MOD & 2) && valid) slope = __ldg(p.slopes + head) * 1.4426950408889634f;
+      const bool idle = __all_sync(0xffffffffu, !valid);  // rows of this warp are nobody's
+      float m_ref = kNegInf, l_sum = 0.f;
+      for (int n = 0; n < n_mine; ++n) {
+        const int j = dual ? n : 2 * n + grp;
+        const int k0 = (d.t0 + j) * kChTile;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[grp], sc & 1));
+        if (!ok) break;
+        ++sc;
+        tc_fence_after();
+        // Slots outside the block's range may hold anything: their V rows become
+        // zeros, so that 0 * V stays 0 (whole pages outside are zeros already).
+        // (DUAL: group 0 does it; group 1's product is issued after group 0's.)
+        const int z0 = min(max(d.lo - k0, 0), kChTile), z1 = min(max(d.hi - k0, 0), kChTile);
+        if ((((z0 | z1) & 15) != 0) && (!dual || grp == 0)) {
+          const unsigned s = seq0 + unsigned(chunk_vseq(j, lag, d.nt));
+          ok = __all_sync(0xffffffffu, mbar_wait(&full[s % NS], (s / NS) & 1));
+          if (!ok) break;
+          const uint32_t vb = smem_u32(tiles + G::kRingOff) + uint32_t(s % NS) * G::kRowTile;
+          const int pad0 = z0 & 15, pad1 = (16 - (z1 & 15)) & 15;
+          for (int c = row; c < (pad0 + pad1) * KB * 8; c += 128) {
+            const int i = c / (KB * 8), rem = c % (KB * 8);
+            const int key = i < pad0 ? z0 - 1 - i : z1 + (i - pad0);
+            st_shared_v4(vb + (key >> 3) * G::kGroupBytes + (rem >> 3) * 1024 + (key & 7) * 128 +
+                             ((rem & 7) << 4), 0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+        }
+        if (!idle) {
+          uint32_t s[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, s[c]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_bind32(s[c]);
+          // Scores in log2 units when they are capped or biased; otherwise the
+          // scale (> 0) waits for the exponent's multiply-add.
+          if constexpr (MOD != 0) {
+            const float d0 = float(k0 - pos);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                float x = __uint_as_float(s[c][e]);
+                if constexpr (MOD & 1)  // cap * tanh(u) = cap - 2 cap / (1 + exp(2 u))
+                  x = fmaf(-2.f * p.cap_log2, fast_rcp(1.f + fast_exp2(x * p.cap_arg)), p.cap_log2);
+                else
+                  x *= p.scale_log2;
+                if constexpr (MOD & 2) x = fmaf(-slope, fabsf(d0 + float(c * 32 + e)), x);
+                s[c][e] = __float_as_uint(x);
+              }
+          }
+          const int a = lo - k0, b = hi - k0;
+          if (!__all_sync(0xffffffffu, a <= 0 && b >= kChTile)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int bc = min(max(b - c * 32, 0), 32), ac = min(max(a - c * 32, 0), 32);
+              const uint32_t below_b = bc == 32 ? 0xffffffffu : (1u << bc) - 1u;
+              const uint32_t below_a = ac == 32 ? 0xffffffffu : (1u << ac) - 1u;
+              const uint32_t bits = below_b & ~below_a;
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!((bits >> e) & 1u)) s[c][e] = __float_as_uint(kNegInf);
+            }
+          }
+          float mx;
+          {
+            float m8[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              m8[i] = fmax3(__uint_as_float(s[0][i]), __uint_as_float(s[0][i + 8]),
+                            __uint_as_float(s[0][i + 16]));
+              m8[i] = fmax3(m8[i], __uint_as_float(s[0][i + 24]), __uint_as_float(s[1][i]));
+#pragma unroll
+              for (int q = 1; q < 4; ++q) {
+                m8[i] = fmax3(m8[i], __uint_as_float(s[q][i + 8]), __uint_as_float(s[q][i + 16]));
+                if (q < 3)
+                  m8[i] = fmax3(m8[i], __uint_as_float(s[q][i + 24]), __uint_as_float(s[q + 1][i]));
+                else
+                  m8[i] = fmaxf(m8[i], __uint_as_float(s[q][i + 24]));
+              }
+            }
+            mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
+          }
+          if constexpr (MOD == 0) mx *= p.scale_log2;  // -inf stays -inf
+          // Lazy maximum: the reference moves only when a row's maximum grows by
+          // more than 2^8, with probabilities up to 2^8 until then.
+          float alpha = 1.f;
+          bool rescale = false;
+          if (mx > m_ref + 8.f) {
+            alpha = fast_exp2(m_ref - mx);
+            rescale = m_ref != kNegInf;
+            m_ref = mx;
+            l_sum *= alpha;
+          }
+          const float mb = m_ref == kNegInf ? 0.f : -m_ref;
+          float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t ph[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              float x0, x1, x2, x3;
+              fma_pair(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]),
+                       MOD ? 1.f : p.scale_log2, mb, x0, x1);
+              fma_pair(__uint_as_float(s[c][e + 2]), __uint_as_float(s[c][e + 3]),
+                       MOD ? 1.f : p.scale_log2, mb, x2, x3);
+              x0 = fast_exp2(x0);
+              x1 = fast_exp2(x1);
+              x2 = fast_exp2(x2);
+              x3 = fast_exp2(x3);
+              add_pair(l0, l1, x0, x1);
+              add_pair(l2, l3, x2, x3);
+              // (P in the input's 16 bits: one rounding of half a step a term, the
+              // A operand's type; the sum l keeps the unrounded values)
+              ph[e / 2] = pack_pair<T>(x0, x1);
+              ph[e / 2 + 1] = pack_pair<T>(x2, x3);
+            }
+            tmem_st16(tS + c * 16, ph);
+          }
+          l_sum += (l0 + l1) + (l2 + l3);
+          // O moves to the new reference. Its last product is complete: this
+          // tile's S was issued after it and has been waited for.
+          if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(tO + c, o);
+              tmem_ld_wait();
+              tmem_bind32(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st32(tO + c, o);
+            }
+          }
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[grp]);
+      }
+      if (!ok) break;
+      seq0 += 2u * unsigned(d.nt);
+
+      // -------------------------------------------------------------- epilogue
+      ok = __all_sync(0xffffffffu, mbar_wait(&o_full[grp], k & 1) &&
+                                       (dual || mbar_wait(&o_full[grp ^ 1], k & 1)));
+      if (!ok) break;
+      tc_fence_after();
+      // The row's factor on each group's O (0 where it saw no key), its columns
+      // [c0, c1), and where they go.
+      float f0, f1 = 0.f, m_out = m_ref, l_out = l_sum;
+      int c0 = 0, c1 = D;
+      if (!dual) {
+        ml_x[grp * 128 + row] = make_float2(m_ref, l_sum);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&xch[grp]);
+        ok = __all_sync(0xffffffffu, mbar_wait(&xch[grp ^ 1], alt & 1));
+        if (!ok) break;
+        const float2 a = ml_x[row], b = ml_x[128 + row];
+        m_out = fmaxf(a.x, b.x);
+        f0 = a.x == kNegInf ? 0.f : fast_exp2(a.x - m_out);
+        f1 = b.x == kNegInf ? 0.f : fast_exp2(b.x - m_out);
+        l_out = f0 * a.y + f1 * b.y;
+        c0 = grp * (D / 2);
+        c1 = c0 + D / 2;
+      } else {
+        f0 = m_ref == kNegInf ? 0.f : 1.f;
+      }
+      if (d.slot < 0) {
+        const float inv = l_out > 0.f ? 1.f / l_out : 0.f;
+        f0 *= inv;
+        f1 *= inv;
+      }
+      const bool two = !dual && d.nt > 1;  // group 1 has products of its own
+      const uint32_t tA = tbase + lane_addr + G::kTmemO + (dual ? uint32_t(grp) * 128 : 0u);
+      if (!idle) {
+        const int prow = (dual ? grp * 128 : 0) + row;
+#pragma unroll 1
+        for (int c = c0; c < c1; c += 32) {
+          uint32_t o[32], o2[32];
+          tmem_ld32(tA + c, o);
+          if (two) tmem_ld32(tA + 128 + c, o2);
+          tmem_ld_wait();
+          tmem_bind32(o);
+          float v[32];
+          if (two) {
+            tmem_bind32(o2);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              v[e] = (f0 != 0.f ? f0 * __uint_as_float(o[e]) : 0.f) +
+                     (f1 != 0.f ? f1 * __uint_as_float(o2[e]) : 0.f);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = f0 != 0.f ? f0 * __uint_as_float(o[e]) : 0.f;
+          }
+          if (valid && d.slot >= 0) {
+            float4* to = p.part_o + (size_t(d.slot) * (D / 4) + c / 4) * p.part_rows + prow;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              to[size_t(e / 4) * p.part_rows] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          } else if (valid) {
+            const size_t at = (size_t(d.first + tok) * p.hq + head) * D + c;
+            if (p.out_f32) {
+              float4* to = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                to[e / 4] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            } else {
+              uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at);
+#pragma unroll
+              for (int e = 0; e < 32; e += 8)
+                to[e / 8] = make_uint4(pack_pair<T>(v[e], v[e + 1]), pack_pair<T>(v[e + 2], v[e + 3]),
+                                       pack_pair<T>(v[e + 4], v[e + 5]), pack_pair<T>(v[e + 6], v[e + 7]));
+            }
+          }
+          __syncwarp();
+        }
+        if (d.slot >= 0 && valid && (dual || grp == 0))
+          p.part_ml[size_t(d.slot) * p.part_rows + prow] = make_float2(m_out, l_out);
+      }
+      tc_fence_before();
+      if (!dual) {  // both groups read both O: neither goes on before the other has
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&xch_done[grp]);
+        ok = __all_sync(0xffffffffu, mbar_wait(&xch_done[grp ^ 1], alt & 1));
+        ++alt;
+        tc_fence_after();
+      }
+    }
+    if (!ok && lane == 0) atomicOr(p.err, kErrTimeout);
+    tc_fence_before();
+    named_barrier_sync(1, kChThreads);
+  }
+}
+
+// Joins the pieces of the item that starts (and does not end) in block
+// blockIdx.x: its own, then those of the following blocks up to the one that
+// ends it, 32 rows per block of blockIdx.y.
 template <int D, typename T>
-__global__ void __launch_bounds__(128) chunk_rows_kernel(const ChunkParams p) {
-  __shared__ float s_q[4][D];
+__global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   grid_launch_dependents();
   grid_dependency_wait();
-  const long long row = (long long)blockIdx.x * 4 + warp;
-  if (row >= (long long)p.tokens * p.hq) return;
-  const int t = int(row / p.hq), h = int(row % p.hq);
-  int lo = 0, hi = p.batch;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.query_start[mid] <= t) lo = mid; else hi = mid;
-  }
-  const ChunkRequest rq = chunk_request(p, lo);
-  if (t < rq.first || t >= rq.first + rq.n) return;
-  const int pos = rq.len - rq.n + (t - rq.first);
-  int end = pos + 1, begin = 0;
-  if (p.prefix) end = max(end, min(p.prefix[lo], rq.len));
-  if (p.window) begin = max(begin, pos + 1 - p.window);
-  if (p.key_start) begin = max(begin, p.key_start[t]);
-  const T* q = static_cast<const T*>(p.q) + t * p.q_stride + size_t(h) * D;
-  for (int d = lane; d < D; d += 32) s_q[warp][d] = float(q[d]);
-  __syncwarp();
-  const int kvh = h / p.group;
-  const float slope = p.slopes ? p.slopes[h] : 0.f;
-  float m = -INFINITY, l = 0.f, acc[D / 32];
+  const int c = blockIdx.x, blocks = gridDim.x;
+  const int* s = p.sched + size_t(c) * 8;
+  if (!s[1]) return;
+  const int first = s[2], ntok = s[3], head = s[4];
+  const int row = blockIdx.y * 32 + lane;
+  const int tok = (row / 128) * p.tile_tokens + (row % 128) / p.group;
+  const bool valid = row < p.part_rows && (row % 128) / p.group < p.tile_tokens && tok < ntok;
+  if (!__any_sync(0xffffffffu, valid)) return;
+  int end = c + 1;  // one past the block that ends the item
+  while (end < blocks && p.sched[size_t(end) * 8] != 2) ++end;
+  end = min(end + 1, blocks);
+  auto none = [&](int i) { return i != c && p.sched[size_t(i) * 8] == 3; };
+  auto slot = [&](int i) -> size_t { return i == c ? size_t(c) * 2 + 1 : size_t(i) * 2; };
+  float m = -INFINITY, l = 0.f;
+  if (valid)
+    for (int i = c; i < end; ++i)
+      if (!none(i)) m = fmaxf(m, p.part_ml[slot(i) * p.part_rows + row].x);
+  constexpr int N = D / 16;  // float4 pieces of a warp
+  float4 acc[N];
 #pragma unroll
-  for (int r = 0; r < D / 32; ++r) acc[r] = 0.f;
-  for (int j0 = begin; j0 < end; j0 += 32) {
-    const int j = j0 + lane;
-    float x = -INFINITY;
-    long long at = -1;
-    if (j < end) {
-      const int page = p.pages[size_t(lo) * p.max_pages + j / kPageSize];
-      x = 0.f;
-      if (page < 0 || page >= p.physical_pages) {
-        atomicOr(p.err, kErrPageRange);
-      } else {
-        at = page * p.block_stride + (j % kPageSize) * p.slot_stride + kvh * p.head_stride;
-        for (int d = 0; d < D; ++d) x += s_q[warp][d] * float(static_cast<const T*>(p.k)[at + d]);
-      }
-      x *= p.scale;
-      if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap);
-      x -= slope * fabsf(float(pos - j));
-    }
-    float mx = x;
-    for (int d = 1; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-    const float mn = fmaxf(m, mx), a = expf(m - mn), w = expf(x - mn);
-    m = mn;
-    l = l * a + w;
+  for (int q = 0; q < N; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (!valid) return;
+  for (int i = c; i < end; ++i) {
+    if (none(i)) continue;
+    const float2 ml = p.part_ml[slot(i) * p.part_rows + row];
+    if (ml.x == -INFINITY) continue;
+    const float w = fast_exp2(ml.x - m);
+    l += w * ml.y;
 #pragma unroll
-    for (int r = 0; r < D / 32; ++r) acc[r] *= a;
-    for (int k = 0; k < min(32, end - j0); ++k) {
-      const float wk = __shfl_sync(0xffffffffu, w, k);
-      const long long ak = __shfl_sync(0xffffffffu, at, k);
-      if (ak < 0) continue;
-#pragma unroll
-      for (int r = 0; r < D / 32; ++r)
-        acc[r] += wk * float(static_cast<const T*>(p.v)[ak + r * 32 + lane]);
+    for (int q = 0; q < N; ++q) {
+      const float4 o = p.part_o[(slot(i) * (D / 4) + warp * N + q) * p.part_rows + row];
+      acc[q].x += w * o.x;
+      acc[q].y += w * o.y;
+      acc[q].z += w * o.z;
+      acc[q].w += w * o.w;
     }
   }
-  for (int d = 1; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
   const float inv = l > 0.f ? 1.f / l : 0.f;
+  const size_t at = (size_t(first + tok) * p.hq + head * p.group + (row % 128) % p.group) * D +
+                    warp * N * 4;
 #pragma unroll
-  for (int r = 0; r < D / 32; ++r) {
-    const size_t o = size_t(row) * D + r * 32 + lane;
+  for (int q = 0; q < N; ++q) {
+    const float4 o = make_float4(acc[q].x * inv, acc[q].y * inv, acc[q].z * inv, acc[q].w * inv);
     if (p.out_f32)
-      static_cast<float*>(p.out)[o] = acc[r] * inv;
+      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at + q * 4) = o;
     else
-      static_cast<T*>(p.out)[o] = T(acc[r] * inv);
+      *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at + q * 4) =
+          make_uint2(pack_pair<T>(o.x, o.y), pack_pair<T>(o.z, o.w));
   }
 }
 

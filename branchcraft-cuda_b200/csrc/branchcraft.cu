@@ -1060,13 +1060,121 @@ uintptr_t address_bits(const T* p, R... rest) {
 }
 
 // A cache whose rows the kernels may copy in 16-byte pieces.
-bool layout_ok(const bc_kv_layout* l) {
-  return l && l->block_stride >= 0 && l->slot_stride > 0 && l->head_stride > 0 &&
+bool layout_ok(const bc_kv_layout* l, int pages) {
+  return l && (l->block_stride > 0 || pages == 1) && l->slot_stride > 0 && l->head_stride > 0 &&
          ((l->block_stride | l->slot_stride | l->head_stride) & 7) == 0;
 }
 
 // Pages whose slots an int can number.
 bool pool_ok(int pages) { return pages >= 1 && pages <= 0x7fffffff / kPageSize; }
+
+bool encode_map_n(CUtensorMap* map, int dtype, int rank, const void* base, const uint64_t* dims,
+                  const uint64_t* strides_bytes, const uint32_t* box) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t gdim[5], gstr[4];
+  cuuint32_t bdim[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    gdim[i] = dims[i];
+    bdim[i] = box[i];
+    estr[i] = 1;
+    if (i + 1 < rank) {
+      if (strides_bytes[i] % 16 || strides_bytes[i] >= (uint64_t(1) << 40)) return false;
+      gstr[i] = strides_bytes[i];
+    }
+  }
+  return fn(map, dtype == BC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+            cuuint32_t(rank), const_cast<void*>(base), gdim, gstr, bdim, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Q [tokens, heads, dim] as (dim, heads, tokens): boxes of one KV head's query
+// heads of a row tile's tokens, 64 dims wide.
+bool encode_rows_map(CUtensorMap* map, int dtype, const void* q, int dim, int heads, int tokens,
+                     long long token_stride, int group, int tile_tokens) {
+  const uint64_t dims[3] = {uint64_t(dim), uint64_t(heads), uint64_t(tokens)};
+  // (one token: any valid stride)
+  const uint64_t st[2] = {uint64_t(dim) * 2,
+                          uint64_t(tokens > 1 ? token_stride : (long long)heads * dim) * 2};
+  const uint32_t box[3] = {64, uint32_t(group), uint32_t(tile_tokens)};
+  return st[1] > 0 && encode_map_n(map, dtype, 3, q, dims, st, box);
+}
+
+// K or V of a paged cache as (64 dims, 8 slots, 64-dim blocks of the heads, 2
+// halves of a page, pages): a box is one head's 16 rows of a page, each half
+// page a run of 8-row groups of its 64-dim blocks.
+bool encode_pages_map(CUtensorMap* map, int dtype, const void* base, const bc_shape* s,
+                      const bc_kv_layout* l) {
+  const int kb = s->dim / 64;
+  const uint64_t dims[5] = {64, 8, uint64_t((s->kv_heads - 1) * (l->head_stride / 64) + kb), 2,
+                            uint64_t(s->physical_pages)};
+  const uint64_t block = uint64_t(s->physical_pages > 1 ? l->block_stride : 16 * l->slot_stride);
+  const uint64_t st[4] = {uint64_t(l->slot_stride) * 2, 128, uint64_t(l->slot_stride) * 16, block * 2};
+  const uint32_t box[5] = {64, 8, uint32_t(kb), 2, 1};
+  return encode_map_n(map, dtype, 5, base, dims, st, box);
+}
+
+bool chunk_shape_ok(const bc_shape* s) {
+  return basic_shape_ok(s) && pool_ok(s->physical_pages) && pool_ok(s->max_pages) &&
+         s->batch <= kChMaxBatch && s->query_heads / s->kv_heads <= 128;
+}
+
+// The launch of a chunk attention, from host-known bounds alone.
+struct ChunkPlan {
+  int blocks;    // thread blocks: one per SM, no more than there can be key tiles
+  int rows;      // rows of a partial state
+  size_t bytes;  // workspace; 0 where no item is long enough to be split
+  ChunkPlan(const bc_shape* s, int tokens, int dev) {
+    const int group = s->query_heads / s->kv_heads, tile = 128 / group;
+    const long long key_tiles = (s->max_pages + kChTile / kPageSize - 1) / (kChTile / kPageSize);
+    const long long items = ((long long)tokens / (2 * tile) + std::min(s->batch, tokens)) * s->kv_heads;
+    blocks = int(std::min<long long>(dev < 0 ? 148 : sm_count(dev), items * key_tiles));
+    rows = tokens <= tile ? (tokens * group + 31) / 32 * 32 : 256;
+    // (cuts fall on multiples of kChMinPiece tiles and leave at least half of
+    // that: an item of kChMinPiece + 1 tiles is never split)
+    bytes = key_tiles <= kChMinPiece + 1
+                ? 0
+                : size_t(blocks) * (2 * size_t(rows) * (s->dim * 4 + 8) + 32);
+  }
+};
+
+template <int D, typename T, int MOD>
+cudaError_t launch_chunk_mod(ChunkParams& p, const CUtensorMap* maps, const ChunkPlan& plan,
+                             int dev, cudaStream_t stream) {
+  auto kern = chunk_mma_kernel<D, T, MOD>;
+  static std::atomic<size_t> smem_of[kMaxDevices];
+  size_t smem = smem_of[dev].load(std::memory_order_relaxed);
+  if (!smem) {
+    // As for the tree kernel: the register split needs the launch budget.
+    cudaFuncAttributes fa;
+    cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+    if (e != cudaSuccess) return e;
+    if (fa.numRegs != kChLaunchRegs) return cudaErrorInvalidDeviceFunction;
+    smem = ChunkGeom<D>::smem_bytes(fa.sharedSizeBytes);
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    if (e != cudaSuccess) return e;
+    smem_of[dev].store(smem, std::memory_order_relaxed);
+  }
+  p.smem_bytes = unsigned(smem);
+  cudaError_t e = launch_dependent(kern, dim3(unsigned(plan.blocks)), kChThreads, smem, stream, p,
+                                   maps[0], maps[1], maps[2]);
+  if (e != cudaSuccess || plan.bytes == 0) return e;
+  return launch_dependent(chunk_merge_kernel<D, T>,
+                          dim3(unsigned(plan.blocks), unsigned((plan.rows + 31) / 32)), 128, 0,
+                          stream, p);
+}
+
+template <int D, typename T>
+cudaError_t launch_chunk(ChunkParams& p, const CUtensorMap* maps, const ChunkPlan& plan,
+                         const bc_chunk_options* o, int dev, cudaStream_t stream) {
+  switch ((o->softcap > 0.f ? 1 : 0) | (o->alibi_slopes ? 2 : 0)) {
+    case 0: return launch_chunk_mod<D, T, 0>(p, maps, plan, dev, stream);
+    case 1: return launch_chunk_mod<D, T, 1>(p, maps, plan, dev, stream);
+    case 2: return launch_chunk_mod<D, T, 2>(p, maps, plan, dev, stream);
+    default: return launch_chunk_mod<D, T, 3>(p, maps, plan, dev, stream);
+  }
+}
 
 template <typename T>
 cudaError_t launch_beam_chunks(const BeamSelectParams& p, int dev, cudaStream_t stream) {
@@ -1142,7 +1250,7 @@ int bc_append_kv(const bc_shape* s, int tokens, const void* k, long long k_strid
                  const int* slot_map, const int* clones, int max_clones, const int* counts,
                  void* stream) {
   if (!s || s->kv_heads < 1 || (s->dim != 64 && s->dim != 128) || !pool_ok(s->physical_pages) ||
-      tokens < 0 || !cache_k || !cache_v || !layout_ok(layout) || max_clones < 0 ||
+      tokens < 0 || !cache_k || !cache_v || !layout_ok(layout, s->physical_pages) || max_clones < 0 ||
       (tokens > 0 && (!k || !v || !slot_map)) || (max_clones > 0 && (!clones || !counts)) ||
       (address_bits(k, v, cache_k, cache_v) % 16) || ((k_stride | v_stride) & 7) ||
       k_stride < 0 || v_stride < 0 || (long long)s->kv_heads * s->dim > 0x7fffff)
@@ -1179,9 +1287,8 @@ int bc_append_kv(const bc_shape* s, int tokens, const void* k, long long k_strid
 }
 
 size_t bc_chunk_workspace_bytes(const bc_shape* s, int tokens) {
-  (void)s;
-  (void)tokens;
-  return 0;
+  if (!chunk_shape_ok(s) || tokens < 1) return 0;
+  return ChunkPlan(s, tokens, current_device()).bytes;
 }
 
 int bc_chunk_attention(const bc_shape* s, int tokens, int dtype, const void* q,
@@ -1189,16 +1296,17 @@ int bc_chunk_attention(const bc_shape* s, int tokens, int dtype, const void* q,
                        const bc_kv_layout* layout, const int* pages, const int* query_start,
                        const int* lengths, const bc_chunk_options* options, void* output,
                        int output_f32, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!basic_shape_ok(s) || !pool_ok(s->physical_pages) || !pool_ok(s->max_pages) || tokens < 0 ||
-      (dtype != BC_F16 && dtype != BC_BF16) || s->query_heads / s->kv_heads > 128 || !q || !k ||
-      !v || !layout_ok(layout) || layout->head_stride % 64 || !pages || !query_start || !lengths ||
-      !options || !output || (address_bits(q, k, v, output) % 16) || (q_stride & 7) ||
-      q_stride < 0 || !(options->scale > 0.f) || std::isinf(options->scale) ||
-      !(options->softcap >= 0.f) || std::isinf(options->softcap) || options->window < 0 ||
-      workspace_bytes < bc_chunk_workspace_bytes(s, tokens) ||
-      (bc_chunk_workspace_bytes(s, tokens) > 0 && (!workspace || address_bits(workspace) % 16)))
+  if (!chunk_shape_ok(s) || tokens < 0 || (dtype != BC_F16 && dtype != BC_BF16) || !q || !k ||
+      !v || !layout_ok(layout, s->physical_pages) || layout->head_stride % 64 || !pages ||
+      !query_start || !lengths || !options || !output || (address_bits(q, k, v, output) % 16) ||
+      (q_stride & 7) || q_stride < 0 || !(options->scale > 0.f) || std::isinf(options->scale) ||
+      !(options->softcap >= 0.f) || std::isinf(options->softcap) || options->window < 0)
     return cudaErrorInvalidValue;
   const int dev = current_device();
+  const ChunkPlan plan(s, std::max(tokens, 1), dev);
+  if (workspace_bytes < plan.bytes ||
+      (plan.bytes > 0 && (!workspace || address_bits(workspace) % 16)))
+    return cudaErrorInvalidValue;
   if (dev < 0) return cudaErrorInvalidDevice;
   unsigned* err = error_word(dev);
   if (!err) return cudaErrorInvalidDevice;
@@ -1209,16 +1317,12 @@ int bc_chunk_attention(const bc_shape* s, int tokens, int dtype, const void* q,
   p.hq = s->query_heads;
   p.hkv = s->kv_heads;
   p.group = s->query_heads / s->kv_heads;
+  p.tile_tokens = 128 / p.group;
   p.max_pages = s->max_pages;
   p.physical_pages = s->physical_pages;
-  p.window = options->window;
-  p.q = q;
-  p.q_stride = q_stride;
-  p.k = k;
-  p.v = v;
-  p.block_stride = layout->block_stride;
-  p.slot_stride = layout->slot_stride;
-  p.head_stride = layout->head_stride;
+  // (a window as wide as the table hides nothing)
+  p.window = options->window < s->max_pages * kPageSize ? options->window : 0;
+  p.head_blocks = int(layout->head_stride / 64);
   p.pages = pages;
   p.query_start = query_start;
   p.lengths = lengths;
@@ -1227,17 +1331,29 @@ int bc_chunk_attention(const bc_shape* s, int tokens, int dtype, const void* q,
   p.slopes = options->alibi_slopes;
   p.out = output;
   p.out_f32 = output_f32;
-  p.scale = options->scale;
-  p.softcap = options->softcap;
+  p.scale_log2 = options->scale * kLog2e;
+  p.cap_log2 = options->softcap * kLog2e;
+  p.cap_arg = options->softcap > 0.f ? 2.f * kLog2e * options->scale / options->softcap : 0.f;
+  p.part_rows = plan.rows;
+  if (plan.bytes > 0) {
+    p.part_o = static_cast<float4*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + size_t(plan.blocks) * 2 * plan.rows * (s->dim / 4));
+    p.sched = reinterpret_cast<int*>(p.part_ml + size_t(plan.blocks) * 2 * plan.rows);
+  }
   p.err = err;
   p.token = next_launch_token();
-  const dim3 grid(unsigned(((long long)tokens * p.hq + 3) / 4));
+  CUtensorMap maps[3];
+  if (!encode_rows_map(&maps[0], dtype, q, s->dim, s->query_heads, tokens, q_stride, p.group,
+                       p.tile_tokens) ||
+      !encode_pages_map(&maps[1], dtype, k, s, layout) ||
+      !encode_pages_map(&maps[2], dtype, v, s, layout))
+    return cudaErrorInvalidValue;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (s->dim == 64)
-    return dtype == BC_F16 ? launch_dependent(chunk_rows_kernel<64, __half>, grid, 128, 0, st, p)
-                           : launch_dependent(chunk_rows_kernel<64, __nv_bfloat16>, grid, 128, 0, st, p);
-  return dtype == BC_F16 ? launch_dependent(chunk_rows_kernel<128, __half>, grid, 128, 0, st, p)
-                         : launch_dependent(chunk_rows_kernel<128, __nv_bfloat16>, grid, 128, 0, st, p);
+    return dtype == BC_F16 ? launch_chunk<64, __half>(p, maps, plan, options, dev, st)
+                           : launch_chunk<64, __nv_bfloat16>(p, maps, plan, options, dev, st);
+  return dtype == BC_F16 ? launch_chunk<128, __half>(p, maps, plan, options, dev, st)
+                         : launch_chunk<128, __nv_bfloat16>(p, maps, plan, options, dev, st);
 }
 
 size_t bc_beam_workspace_bytes(int batch, int beams, int vocab, int k) {
