@@ -22,9 +22,14 @@
 // not depend on timing.
 //
 // Warps: 0-3 and 4-7 softmax groups 0 and 1 (thread = row = TMEM lane), 8 the
-// scheduler (item descriptors, Q), 9 the MMA issuer, 10 and 11 the K/V producers
-// (alternate tiles of one ring, eight 16-row boxes each). TMEM: S of group g at
-// 128 g (P over its own S in 16-bit pairs), O of group g at 256 + 128 g.
+// scheduler (item descriptors, Q), 9 the issuer of S = Q K^T, 11 of O += P V, 10 the
+// K/V producer (a ring each, eight 16-row boxes a tile). TMEM holds one S (128
+// columns) that the groups use in turn, P of each group (64, 16-bit pairs) and O of
+// each (128). A group keeps S only while it loads its scores into registers, so the
+// next S, of the other group, is computed beside its exponentials, and a group's own
+// next scores wait for it when it is done. (With a P over each group's own S, S had
+// to wait for the softmax and P V: 3800 cycles a key tile and pair of row tiles, the
+// softmaxes and products in turns; their sums are 2048 each.)
 #pragma once
 
 #include <cuda_bf16.h>
@@ -40,6 +45,7 @@ constexpr int kChTile = 128;      // keys of a tile: eight pages
 constexpr int kChDescs = 4;       // item descriptors in flight
 constexpr int kChMaxBatch = 16384;
 constexpr int kChMinPiece = 4;    // key tiles: the granularity of cuts inside an item
+constexpr int kChItemCost = 3;    // what an item costs beside its key tiles, in key tiles
 // Registers: launched at 168 a thread (65,536 / 384, in eights); the softmax
 // groups grow to 208 (a row's 128 scores stay in registers), the others shrink
 // to 88: together the launch's total.
@@ -130,9 +136,11 @@ struct ChunkGeom {
   static constexpr int kRowTile = 128 * D * 2;   // Q of a row tile, K or V of a key tile
   static constexpr int kPageBytes = 16 * D * 2;
   static constexpr int kGroupBytes = KB * 1024;  // eight keys
-  static constexpr int kStages = D == 128 ? 5 : 8;
+  // rings: S = Q K^T runs up to a tile ahead of O += P V and frees K first
+  static constexpr int kKStages = D == 128 ? 3 : 4, kVStages = D == 128 ? 2 : 4;
+  static constexpr int kStages = kKStages + kVStages;
   // barriers and small state lie before the 1024-byte aligned tiles
-  static constexpr int kBars = 2 * kStages + 2 + 10 + 2 * kChDescs + 1;
+  static constexpr int kBars = 2 * kStages + 3 + 14 + 2 * kChDescs;
   static constexpr int kMiscBytes = kBars * 8 + 16 + kChDescs * int(sizeof(ChunkDesc));
   static constexpr int kQOff = 0;
   static constexpr int kRingOff = 2 * kRowTile;
@@ -145,7 +153,8 @@ struct ChunkGeom {
     const size_t at = (fixed + 15) / 16 * 16;
     return (at + kMiscBytes + 1023) / 1024 * 1024 - at + kTileBytes;
   }
-  static constexpr uint32_t kTmemO = 256, kTmemCols = 512;
+  // TMEM columns: S, P of group g, O of group g
+  static constexpr uint32_t kTmemP = 128, kTmemO = 256, kTmemCols = 512;
 };
 
 // 5-D tiled load: one page's 16 rows of one head as [2][KB][8][128 bytes], so
@@ -193,6 +202,24 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   return r;
 }
 
+// 32 lanes x 8 columns of tensor memory, as tmem_ld32 and its companions.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+                 "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_bind8(uint32_t (&r)[8]) {
+  asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                    "+r"(r[6]), "+r"(r[7]));
+}
+
 // Two FP32 lanes in one instruction: (a0, a1) * (b, b) + (c, c).
 __device__ __forceinline__ void fma_pair(float a0, float a1, float b, float c, float& d0,
                                          float& d1) {
@@ -210,11 +237,31 @@ __device__ __forceinline__ void add_pair(float& a0, float& a1, float b0, float b
       : "f"(b0), "f"(b1));
 }
 
-// The place of K or V tile j of an item of nt tiles in the ring's order: `lag`
-// K tiles first (one for DUAL items, whose first two products share it; two for
-// ALT), then V and K in turn, then the V tiles left over.
-__device__ __forceinline__ int chunk_kseq(int j, int lag) { return j < lag ? j : 2 * j - lag + 1; }
-__device__ __forceinline__ int chunk_vseq(int j, int lag, int nt) { return min(j + lag, nt) + j; }
+// 32 bytes at once (the address a multiple of 32).
+__device__ __forceinline__ void st_global_v8(void* to, uint32_t a, uint32_t b, uint32_t c,
+                                             uint32_t d, uint32_t e, uint32_t f, uint32_t g,
+                                             uint32_t h) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(a), "r"(b),
+               "r"(c), "r"(d), "r"(e), "r"(f), "r"(g), "r"(h)
+               : "memory");
+}
+
+// The order of an item's copies: two K tiles first, then V and K in turn, then the
+// V tiles left over. The tile at place i:
+__device__ __forceinline__ int chunk_tile(int i, int nt, bool& is_v) {
+  const int lead = min(2, nt);
+  if (i < lead) {
+    is_v = false;
+    return i;
+  }
+  i -= lead;
+  if (i < 2 * (nt - lead)) {
+    is_v = (i & 1) == 0;
+    return is_v ? i >> 1 : (i >> 1) + lead;
+  }
+  is_v = true;
+  return i - (nt - lead);
+}
 
 // MOD: bit 0 the tanh cap, bit 1 the distance bias.
 template <int D, typename T, int MOD>
@@ -223,7 +270,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
                      const __grid_constant__ CUtensorMap kmap,
                      const __grid_constant__ CUtensorMap vmap) {
   using G = ChunkGeom<D>;
-  constexpr int KB = G::KB, NS = G::kStages;
+  constexpr int KB = G::KB, NK = G::kKStages, NV = G::kVStages;
   constexpr float kNegInf = -INFINITY;
   constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
   constexpr uint32_t kIdescS = umma_idesc_f16(128, kChTile, false, false) | kBf16;
@@ -232,20 +279,24 @@ __global__ void __launch_bounds__(kChThreads, 1)
   extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + G::kMiscBytes + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem_raw);  // [NS] K or V tile landed
-  uint64_t* empty = full + NS;                             // [NS] its products are done
-  uint64_t* q_full = empty + NS;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem_raw);  // [NK] a K tile landed
+  uint64_t* k_empty = k_full + NK;      // [NK] its S products are done
+  uint64_t* v_full = k_empty + NK;      // [NV]
+  uint64_t* v_empty = v_full + NV;      // [NV] its P V products are done
+  uint64_t* q_full = v_empty + NV;
   uint64_t* q_free = q_full + 1;        // the item's S products are done
-  uint64_t* s_full = q_free + 1;        // [2] S of group g
-  uint64_t* p_full = s_full + 2;        // [2] P of group g written (4 warps)
-  uint64_t* o_full = p_full + 2;        // [2] the item's last product of group g
-  uint64_t* xch = o_full + 2;           // [2] ALT: group g's (m, l) written (4 warps)
+  uint64_t* s_free = q_free + 1;        // S is in its group's registers (4 warps)
+  uint64_t* s_full = s_free + 1;        // [2] S holds scores of group g
+  uint64_t* p_half = s_full + 2;        // [2] P of group g written: the first 64 keys (4 warps)
+  uint64_t* p_full = p_half + 2;        // [2] and the others
+  uint64_t* p_done = p_full + 2;        // [2] its product is complete: P free, O up to date
+  uint64_t* xch = p_done + 2;           // [2] ALT: group g's (m, l) written (4 warps)
   uint64_t* xch_done = xch + 2;         // [2] ALT: group g has read both O (4 warps)
-  uint64_t* desc_full = xch_done + 2;   // [kChDescs]
+  uint64_t* fin = xch_done + 2;         // [2] an issuer's last product
+  uint64_t* desc_full = fin + 2;        // [kChDescs]
   uint64_t* desc_empty = desc_full + kChDescs;  // [kChDescs] read by 11 warps
-  uint64_t* fin = desc_empty + kChDescs;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin + 1);
-  ChunkDesc* descs = reinterpret_cast<ChunkDesc*>(reinterpret_cast<uint8_t*>(fin + 1) + 16);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(desc_empty + kChDescs);
+  ChunkDesc* descs = reinterpret_cast<ChunkDesc*>(reinterpret_cast<uint8_t*>(desc_empty + kChDescs) + 16);
   float2* ml_x = reinterpret_cast<float2*>(tiles + G::kMlOff);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -255,24 +306,30 @@ __global__ void __launch_bounds__(kChThreads, 1)
   }
   if (tid == 0) {
     s_launch_token = p.token;
-    for (int s = 0; s < NS; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+    for (int s = 0; s < NK; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < NV; ++s) {
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
     }
     mbar_init(q_full, 1);
     mbar_init(q_free, 1);
+    mbar_init(s_free, 4);
     for (int g = 0; g < 2; ++g) {
       mbar_init(&s_full[g], 1);
+      mbar_init(&p_half[g], 4);
       mbar_init(&p_full[g], 4);
-      mbar_init(&o_full[g], 1);
+      mbar_init(&p_done[g], 1);
       mbar_init(&xch[g], 4);
       mbar_init(&xch_done[g], 4);
+      mbar_init(&fin[g], 1);
     }
     for (int s = 0; s < kChDescs; ++s) {
       mbar_init(&desc_full[s], 1);
       mbar_init(&desc_empty[s], 11);
     }
-    mbar_init(fin, 1);
     fence_mbar_init();
   }
   if (warp == 9) {
@@ -287,7 +344,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
   grid_launch_dependents();  // (TMEM is allocated: a waiting successor cannot hold it back)
   grid_dependency_wait();
 
-  // ---- plan: key tiles of every request (per KV head), into the idle ring
+  // ---- plan: the cost of every request (per KV head), into the idle ring
   const int block_tokens = 2 * p.tile_tokens;
   long long* tot = reinterpret_cast<long long*>(tiles + G::kRingOff);
   for (int base = warp * 32; base < p.batch; base += (kChThreads / 32) * 32) {
@@ -298,7 +355,8 @@ __global__ void __launch_bounds__(kChThreads, 1)
     long long sum = 0;
     if (nblk <= 4)
       for (int j = 0; j < nblk; ++j)
-        sum += chunk_range(p, r, j * block_tokens, min(block_tokens, r.n - j * block_tokens)).tiles;
+        sum += kChItemCost +
+               chunk_range(p, r, j * block_tokens, min(block_tokens, r.n - j * block_tokens)).tiles;
     for (unsigned many = __ballot_sync(0xffffffffu, nblk > 4); many; many &= many - 1) {
       const int src = __ffs(many) - 1;  // a long chunk: its blocks spread over the warp
       const ChunkRequest o = {__shfl_sync(0xffffffffu, r.first, src),
@@ -307,7 +365,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
                               __shfl_sync(0xffffffffu, r.prefix, src)};
       long long part = 0;
       for (int i0 = lane * block_tokens; i0 < o.n; i0 += 32 * block_tokens)
-        part += chunk_range(p, o, i0, min(block_tokens, o.n - i0)).tiles;
+        part += kChItemCost + chunk_range(p, o, i0, min(block_tokens, o.n - i0)).tiles;
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
       if (lane == src) sum = part;
@@ -333,22 +391,25 @@ __global__ void __launch_bounds__(kChThreads, 1)
         const long long up = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += up;
       }
-      const long long per_head = __shfl_sync(0xffffffffu, incl, 31);
-      const long long units = per_head * p.hkv;
+      const long long cost = __shfl_sync(0xffffffffu, incl, 31) * p.hkv;  // of the whole call
       const long long pre = incl - mine;
-      // Cuts inside an item fall on multiples of `grain` tiles from its start
-      // (an eighth of a share, at least kChMinPiece: a piece costs its partial
+      // Cuts inside an item fall on multiples of `grain` tiles from its start (a
+      // thirty-second of a share, at least kChMinPiece: a piece costs its partial
       // state's way through memory) or on its ends.
-      const long long share = units / gridDim.x;
-      const int grain = int(max((long long)kChMinPiece, min(share / 8, 1ll << 20)));
-      int req = 0, blk = 0, head = 0, off = 0, n_tiles = 1;
+      const long long share = cost / gridDim.x;
+      const int grain = int(max((long long)kChMinPiece, min(share / 32, 1ll << 20)));
+      // A place in the sequence of key tiles: tile `off` of an item.
+      int req = p.batch, blk = 0, head = 0, off = 0;
       ChunkRequest r = {0, 0, 0, 0};
       ChunkRange g = {0, 0, 0, 1};
-      auto cut = [&](long long u) -> long long {  // finds unit u and moves it to a cut
-        if (u <= 0 || u >= units) {
-          if (u >= units) return units;
-          u = 0;
-        }
+      auto load_block = [&] {  // the current block's range
+        g = chunk_range(p, r, blk * block_tokens,
+                        min(block_tokens, r.n - blk * block_tokens));
+      };
+      auto cut = [&](long long u) {  // the place of cost u (the call's end: request p.batch)
+        off = head = blk = 0;
+        req = p.batch;
+        if (u >= cost) return;
         const unsigned below = __ballot_sync(0xffffffffu, mine > 0 && pre * p.hkv <= u);
         const int src = 31 - __clz(below);
         int found = 0;
@@ -359,10 +420,11 @@ __global__ void __launch_bounds__(kChThreads, 1)
         long long rem = u - __shfl_sync(0xffffffffu, at, src) * p.hkv;
         r = chunk_request(p, req);
         const int nblk = (r.n + block_tokens - 1) / block_tokens;
+        int n = 1;
         for (int j0 = 0;; j0 += 32) {  // the block among the request's
           const int j = j0 + lane;
-          const int t = j < nblk ? chunk_range(p, r, j * block_tokens,
-                                               min(block_tokens, r.n - j * block_tokens)).tiles
+          const int t = j < nblk ? kChItemCost + chunk_range(p, r, j * block_tokens,
+                                                             min(block_tokens, r.n - j * block_tokens)).tiles
                                  : 0;
           long long in = t;
 #pragma unroll
@@ -374,26 +436,18 @@ __global__ void __launch_bounds__(kChThreads, 1)
           if (after) {
             const int w = __ffs(after) - 1;
             blk = j0 + w;
-            n_tiles = __shfl_sync(0xffffffffu, t, w);
-            rem -= (__shfl_sync(0xffffffffu, in, w) - n_tiles) * p.hkv;
+            n = __shfl_sync(0xffffffffu, t, w);
+            rem -= (__shfl_sync(0xffffffffu, in, w) - n) * p.hkv;
             break;
           }
           rem -= __shfl_sync(0xffffffffu, in, 31) * p.hkv;
         }
-        head = int(rem / n_tiles);
-        off = int(rem % n_tiles);
-        const int was = off;
+        head = int(rem / n);
+        off = max(int(rem % n) - kChItemCost, 0);
+        n -= kChItemCost;
         off = (off + grain / 2) / grain * grain;
-        if (off > 0 && n_tiles - off < (grain + 1) / 2) off = n_tiles;
-        return u - was + off;
-      };
-      const long long u1 = cut(units * (blockIdx.x + 1) / gridDim.x);
-      const long long u0 = cut(units * blockIdx.x / gridDim.x);
-      long long left = u0 < units ? u1 - u0 : 0;
-      auto load_block = [&] {  // the current block's range
-        g = chunk_range(p, r, blk * block_tokens,
-                        min(block_tokens, r.n - blk * block_tokens));
-        n_tiles = g.tiles;
+        if (off > 0 && n - off < (grain + 1) / 2) off = n;
+        load_block();
       };
       auto next_item = [&] {
         off = 0;
@@ -412,18 +466,27 @@ __global__ void __launch_bounds__(kChThreads, 1)
               break;
             }
           }
+          req = min(req, p.batch);
           if (req < p.batch) r = chunk_request(p, req);
         }
         if (req < p.batch) load_block();
       };
+      // This block's share: from its own cut up to the next block's.
+      cut(cost * (blockIdx.x + 1) / gridDim.x);
+      if (req < p.batch && off >= g.tiles) next_item();
+      const int e_req = req, e_blk = blk, e_head = head, e_off = off;
+      cut(cost * blockIdx.x / gridDim.x);
+      if (req < p.batch && off >= g.tiles) next_item();
+      // tiles of the current item that are this block's, from `off` on
+      auto mine_here = [&]() -> int {
+        if (req >= p.batch) return 0;
+        return (req == e_req && blk == e_blk && head == e_head ? e_off : g.tiles) - off;
+      };
+      int left = mine_here();
       // for the merge: the first piece continues an item that goes on (1) or ends
       // (2) here, or this block has no share (3); and the item that starts here
       // and goes on
       int cont = left > 0 ? 0 : 3, has = 0, h_first = 0, h_ntok = 0, h_head = 0;
-      if (left > 0) {
-        load_block();
-        if (off >= n_tiles) next_item();
-      }
       int k = 0;
       bool q_pending = false;
       for (;; ++k) {
@@ -440,9 +503,9 @@ __global__ void __launch_bounds__(kChThreads, 1)
           d.request = req;
           d.head = head;
           d.t0 = g.t0 + off;
-          d.nt = int(min((long long)(n_tiles - off), left));
+          d.nt = left;
           d.dual = d.ntok > p.tile_tokens;
-          const bool whole = off == 0 && d.nt == n_tiles;
+          const bool whole = off == 0 && d.nt == g.tiles;
           d.slot = whole ? -1 : int(blockIdx.x) * 2 + (off == 0 ? 1 : 0);
           if (!whole && off == 0) {
             has = 1;
@@ -450,7 +513,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
             h_ntok = d.ntok;
             h_head = head;
           }
-          if (off > 0) cont = off + d.nt == n_tiles ? 2 : 1;
+          if (off > 0) cont = off + d.nt == g.tiles ? 2 : 1;
         }
         const int ds = k % kChDescs;
         if (k >= kChDescs)
@@ -476,8 +539,12 @@ __global__ void __launch_bounds__(kChThreads, 1)
         }
         __syncwarp();
         q_pending = true;
-        left -= d.nt;
-        if (left > 0) next_item();
+        if (off + d.nt < g.tiles) {  // the share ends inside this item
+          left = 0;
+        } else {
+          next_item();
+          left = mine_here();
+        }
       }
       if (p.sched && lane == 0) {
         int* s = p.sched + size_t(blockIdx.x) * 8;
@@ -488,13 +555,20 @@ __global__ void __launch_bounds__(kChThreads, 1)
         s[4] = h_head;
       }
       if (!ok && q_pending) mbar_drain(q_full, (k - (k > 0)) & 1);
-    } else if (warp == 9) {
-      // -------------------------------------------------------------- MMAs
+    } else if (warp != 10) {
+      // ------------------------------------------------------------ issuers
+      // Warp 9: S_g = Q_g K^T, warp 11: O_g += P_g V, the groups in turn. (A
+      // tcgen05.mma holds its issuing thread for about its own run time: the gaps
+      // of one issuer, barriers and commits, are the other's.) Every barrier is
+      // waited for phase by phase.
+      const bool is_pv = warp == 11;
       const uint64_t qdesc = umma_desc_sw128(smem_u32(tiles + G::kQOff), 16, 1024);
-      const uint64_t kdesc0 = umma_desc_sw128(smem_u32(tiles + G::kRingOff), 16, G::kGroupBytes);
-      const uint64_t vdesc0 = umma_desc_sw128(smem_u32(tiles + G::kRingOff), 1024, G::kGroupBytes);
-      unsigned seq0 = 0;           // ring place of the item's first tile
-      uint32_t pc[2] = {0u, 0u};   // P tiles taken of each group
+      const uint64_t kdesc = umma_desc_sw128(smem_u32(tiles + G::kRingOff), 16, G::kGroupBytes);
+      const uint64_t vdesc = umma_desc_sw128(
+          smem_u32(tiles + G::kRingOff + NK * G::kRowTile), 1024, G::kGroupBytes);
+      const bool leader = elect_one();  // issues every product and commit
+      unsigned tile = 0, count = 0;     // tiles of the ring, products issued
+      uint32_t pc[2] = {0u, 0u};        // P tiles taken of each group
       for (int k = 0; ok; ++k) {
         const int ds = k % kChDescs;
         ok = __all_sync(0xffffffffu, mbar_wait(&desc_full[ds], (k / kChDescs) & 1));
@@ -503,78 +577,74 @@ __global__ void __launch_bounds__(kChThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&desc_empty[ds]);
         if (end) break;
-        const int lag = dual ? 1 : 2;
-        const int n_of[2] = {dual ? nt : (nt + 1) / 2, dual ? nt : nt / 2};
-        ok = __all_sync(0xffffffffu, mbar_wait(q_full, k & 1));
+        if (!is_pv) ok = __all_sync(0xffffffffu, mbar_wait(q_full, k & 1));
         if (!ok) break;
-        for (int n = 0; n <= n_of[0] && ok; ++n) {
+        for (int j = 0; j < nt && ok; ++j, ++tile) {
+          const int st = int(tile % (is_pv ? NV : NK));
+          ok = __all_sync(0xffffffffu, is_pv ? mbar_wait(&v_full[st], (tile / NV) & 1)
+                                             : mbar_wait(&k_full[st], (tile / NK) & 1));
+          if (!ok) break;
+#pragma unroll 1
+          for (int g = dual ? 0 : (j & 1); g <= (dual ? 1 : (j & 1)); ++g, ++count) {
+            if (is_pv) {
+              const uint32_t par = (g ? pc[1] : pc[0]) & 1;
+              if (g) ++pc[1]; else ++pc[0];
+              const uint64_t vd = vdesc + uint64_t((st * G::kRowTile) >> 4);
+              const uint32_t acc = (dual ? j : j >> 1) > 0 ? 1u : 0u;
+              // (the first half's products run while the second half of P is
+              // still being made)
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            if (n > 0 && n - 1 < n_of[g] && ok) {  // O_g += P_g V
-              const int j = dual ? n - 1 : 2 * (n - 1) + g;
-              const unsigned s = seq0 + unsigned(chunk_vseq(j, lag, nt));
-              const int st = int(s % NS);
-              ok = __all_sync(0xffffffffu, mbar_wait(&p_full[g], pc[g] & 1) &&
-                                               mbar_wait(&full[st], (s / NS) & 1));
-              if (!ok) break;
-              ++pc[g];
-              tc_fence_after();
-              const uint64_t vd = vdesc0 + uint64_t((st * G::kRowTile) >> 4);
+              for (int h = 0; h < 2; ++h) {
+                ok = __all_sync(0xffffffffu, mbar_wait(h ? &p_full[g] : &p_half[g], par));
+                if (!ok) break;
+                tc_fence_after();
+                if (leader) {
 #pragma unroll
-              for (int kk = 0; kk < kChTile / 16; ++kk)
-                if (elect_one())
-                  umma_f16_ts(tbase + G::kTmemO + g * 128, tbase + g * 128 + kk * 8,
-                              vd + uint64_t((kk * 2 * G::kGroupBytes) >> 4), kIdescPV,
-                              (n > 1 || kk > 0) ? 1u : 0u);
-              if (elect_one()) {
-                if (!dual || g == 1) umma_commit(&empty[st]);
-                if (n == n_of[g]) umma_commit(&o_full[g]);
+                  for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+                    umma_f16_ts(tbase + G::kTmemO + g * 128, tbase + G::kTmemP + g * 64 + kk * 8,
+                                vd + uint64_t((kk * 2 * G::kGroupBytes) >> 4), kIdescPV,
+                                kk > 0 ? 1u : acc);
+                  if (h) {
+                    umma_commit(&p_done[g]);
+                    if (!dual || g == 1) umma_commit(&v_empty[st]);
+                  }
+                }
+                __syncwarp();
               }
-              __syncwarp();
-            }
-            if (n < n_of[g] && ok) {  // S_g = Q_g K^T (over the P just read)
-              const int j = dual ? n : 2 * n + g;
-              const unsigned s = seq0 + unsigned(chunk_kseq(j, lag));
-              const int st = int(s % NS);
-              ok = __all_sync(0xffffffffu, mbar_wait(&full[st], (s / NS) & 1));
+              if (!ok) break;
+            } else {
+              // S is free once the last group holds its scores in registers
+              if (count > 0) ok = __all_sync(0xffffffffu, mbar_wait(s_free, (count - 1) & 1));
               if (!ok) break;
               tc_fence_after();
               const uint64_t qd = qdesc + uint64_t((dual ? g * G::kRowTile : 0) >> 4);
-              const uint64_t kd = kdesc0 + uint64_t((st * G::kRowTile) >> 4);
+              const uint64_t kd = kdesc + uint64_t((st * G::kRowTile) >> 4);
+              if (leader) {
 #pragma unroll
-              for (int ks = 0; ks < D / 16; ++ks)
-                if (elect_one())
-                  umma_f16(tbase + g * 128, qd + uint64_t(((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4),
+                for (int ks = 0; ks < D / 16; ++ks)
+                  umma_f16(tbase, qd + uint64_t(((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4),
                            kd + uint64_t(((ks >> 2) * 1024 + (ks & 3) * 32) >> 4), kIdescS,
                            ks > 0 ? 1u : 0u);
-              if (elect_one()) {
                 umma_commit(&s_full[g]);
-                if (!dual || g == 1) umma_commit(&empty[st]);
-                // the item's last S product: of group 1 when it has as many tiles
-                if (n == n_of[0] - 1 && (g == 1 || n_of[1] < n_of[0])) umma_commit(q_free);
+                if (!dual || g == 1) {
+                  umma_commit(&k_empty[st]);
+                  if (j == nt - 1) umma_commit(q_free);
+                }
               }
-              __syncwarp();
             }
+            __syncwarp();
           }
         }
-        // (an ALT item of one tile has no product of group 1)
-        if (ok && n_of[1] == 0) {
-          if (elect_one()) umma_commit(&o_full[1]);
-          __syncwarp();
-        }
-        seq0 += 2u * unsigned(nt);
       }
-      if (elect_one()) umma_commit(fin);
+      if (leader) umma_commit(&fin[is_pv]);
       __syncwarp();
-      if (lane == 0) mbar_drain(fin, 0);
+      if (lane == 0) mbar_drain(&fin[is_pv], 0);
       __syncwarp();
     } else {
-      // ---------------------------------------------------------- producers
-      // Ring places of parity `par`; lane l holds the page id of page (l & 7) of
-      // this warp's step 4 batch + l / 8, loaded a batch ahead.
-      const int par = warp - 10;
-      unsigned seq0 = 0, last = 0;
-      bool any = false;
+      // ----------------------------------------------------------- producer
+      // Lane l holds the page id of page (l & 7) of ring place 4 batch + l / 8,
+      // loaded a batch ahead.
+      unsigned tile0 = 0, k_next = 0, v_next = 0;  // first tile of the item; tiles issued
       for (int k = 0; ok; ++k) {
         const int ds = k % kChDescs;
         ok = __all_sync(0xffffffffu, mbar_wait(&desc_full[ds], (k / kChDescs) & 1));
@@ -583,26 +653,13 @@ __global__ void __launch_bounds__(kChThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&desc_empty[ds]);
         if (d.end) break;
-        const int nt = d.nt, lag = min(d.dual ? 1 : 2, nt), steps = nt;  // of 2 nt places
+        const int nt = d.nt, steps = 2 * nt;
         const int* row = p.pages + size_t(d.request) * p.max_pages;
-        auto tile_of = [&](int s, bool& is_v) -> int {  // ring place -> tile
-          if (s < lag) {
-            is_v = false;
-            return s;
-          }
-          s -= lag;
-          if (s < 2 * (nt - lag)) {
-            is_v = (s & 1) == 0;
-            return is_v ? s >> 1 : (s >> 1) + lag;
-          }
-          is_v = true;
-          return s - (nt - lag);
-        };
         auto load_id = [&](int first) -> int {
           const int i = first + (lane >> 3);
           if (i >= steps) return -1;
           bool is_v;
-          const int pg = (d.t0 + tile_of(par + 2 * i, is_v)) * (kChTile / kPageSize) + (lane & 7);
+          const int pg = (d.t0 + chunk_tile(i, nt, is_v)) * (kChTile / kPageSize) + (lane & 7);
           // pages that no row of the block sees stay out: the copy fills zeros
           if (pg * kPageSize >= d.hi || (pg + 1) * kPageSize <= d.lo) return -1;
           const int id = __ldg(row + pg);
@@ -618,29 +675,32 @@ __global__ void __launch_bounds__(kChThreads, 1)
             cur = nxt;
             nxt = load_id(i + 4);
           }
-          const unsigned s = seq0 + unsigned(par + 2 * i);
-          const int st = int(s % NS);
-          if (s >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], ((s / NS) - 1) & 1));
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&full[st], uint32_t(G::kRowTile));
-          const int id = __shfl_sync(0xffffffffu, cur, (i & 3) * 8 + (lane & 7));
           bool is_v;
-          tile_of(par + 2 * i, is_v);
+          const unsigned s = tile0 + unsigned(chunk_tile(i, nt, is_v));
+          const int st = int(s % (is_v ? NV : NK));
+          uint64_t* full = (is_v ? v_full : k_full) + st;
+          if (s >= (is_v ? NV : NK))
+            ok = __all_sync(0xffffffffu, is_v ? mbar_wait(&v_empty[st], ((s / NV) - 1) & 1)
+                                              : mbar_wait(&k_empty[st], ((s / NK) - 1) & 1));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(full, uint32_t(G::kRowTile));
+          const int id = __shfl_sync(0xffffffffu, cur, (i & 3) * 8 + (lane & 7));
           if (lane < 8)
-            tma_load_5d(tiles + G::kRingOff + st * G::kRowTile + lane * G::kPageBytes,
-                        is_v ? &vmap : &kmap, &full[st], 0, 0, d.head * p.head_blocks, 0, id);
+            tma_load_5d(tiles + G::kRingOff + ((is_v ? NK : 0) + st) * G::kRowTile +
+                            lane * G::kPageBytes,
+                        is_v ? &vmap : &kmap, full, 0, 0, d.head * p.head_blocks, 0, id);
           __syncwarp();
-          last = s;
-          any = true;
+          (is_v ? v_next : k_next) = s + 1;
         }
-        seq0 += 2u * unsigned(nt);
+        tile0 += unsigned(nt);
       }
-      if (!ok && any)  // this warp's copies in flight: its last places
-        for (unsigned s = last; last - s < NS; s -= 2) {
-          if (lane == 0) mbar_drain(&full[s % NS], (s / NS) & 1);
-          __syncwarp();
-          if (s < 2) break;
-        }
+      if (!ok && lane == 0) {  // copies in flight: each ring's last tiles
+        for (unsigned s = k_next - min(k_next, unsigned(NK)); s < k_next; ++s)
+          mbar_drain(&k_full[s % NK], (s / NK) & 1);
+        for (unsigned s = v_next - min(v_next, unsigned(NV)); s < v_next; ++s)
+          mbar_drain(&v_full[s % NV], (s / NV) & 1);
+      }
+      __syncwarp();
     }
     if (!ok && lane == 0) atomicOr(p.err, kErrTimeout);
     tc_fence_before();
@@ -657,21 +717,20 @@ __global__ void __launch_bounds__(kChThreads, 1)
     regs_increase<kChSoftmaxRegs>();
     const int grp = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
-    const uint32_t tS = tbase + lane_addr + uint32_t(grp) * 128;
+    const uint32_t tS = tbase + lane_addr;
+    const uint32_t tP = tbase + lane_addr + G::kTmemP + uint32_t(grp) * 64;
     const uint32_t tO = tbase + lane_addr + G::kTmemO + uint32_t(grp) * 128;
     const int row_tok = row / p.group, row_head = row % p.group;
-    uint32_t sc = 0, alt = 0;  // S tiles taken; ALT items done
-    unsigned seq0 = 0;
+    uint32_t sc = 0, alt = 0;  // tiles of this group, ALT items done
+    unsigned tile0 = 0;        // the item's first tile in the rings
     for (int k = 0; ok; ++k) {
       const int ds = k % kChDescs;
       ok = __all_sync(0xffffffffu, mbar_wait(&desc_full[ds], (k / kChDescs) & 1));
       if (!ok) break;
-      const ChunkDesc d = descs[ds];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&desc_empty[ds]);
+      // (held until the item's end: its fields are read where they are needed)
+      const volatile ChunkDesc& d = descs[ds];
       if (d.end) break;
       const bool dual = d.dual != 0;
-      const int lag = dual ? 1 : 2;
       const int n_mine = dual ? d.nt : (d.nt + 1 - grp) / 2;
       const int tok = (dual ? grp * p.tile_tokens : 0) + row_tok;
       const bool valid = row_tok < p.tile_tokens && tok < d.ntok;
@@ -689,150 +748,178 @@ __global__ void __launch_bounds__(kChThreads, 1)
       if ((MOD & 2) && valid) slope = __ldg(p.slopes + head) * 1.4426950408889634f;
       const bool idle = __all_sync(0xffffffffu, !valid);  // rows of this warp are nobody's
       float m_ref = kNegInf, l_sum = 0.f;
-      for (int n = 0; n < n_mine; ++n) {
+      // Slots outside the block's range may hold anything: their V rows become
+      // zeros, so that 0 * V stays 0 (whole pages outside are zeros already).
+      // (DUAL: both groups do, each before its own product.)
+      auto zero_pads = [&](int j, int k0) -> bool {
+        const int z0 = min(max(d.lo - k0, 0), kChTile), z1 = min(max(d.hi - k0, 0), kChTile);
+        if (((z0 | z1) & 15) == 0) return true;
+        const unsigned vt = tile0 + unsigned(j);
+        if (!__all_sync(0xffffffffu, mbar_wait(&v_full[vt % NV], (vt / NV) & 1))) return false;
+        const uint32_t vb = smem_u32(tiles + G::kRingOff) + uint32_t(NK + vt % NV) * G::kRowTile;
+        const int pad0 = z0 & 15, pad1 = (16 - (z1 & 15)) & 15;
+        for (int c = row; c < (pad0 + pad1) * KB * 8; c += 128) {
+          const int i = c / (KB * 8), rem = c % (KB * 8);
+          const int key = i < pad0 ? z0 - 1 - i : z1 + (i - pad0);
+          st_shared_v4(vb + (key >> 3) * G::kGroupBytes + (rem >> 3) * 1024 + (key & 7) * 128 +
+                           ((rem & 7) << 4), 0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+        return true;
+      };
+      if (idle) {  // nothing to compute: the barriers alone
+        for (int n = 0; n < n_mine && ok; ++n, ++sc) {
+          const int j = dual ? n : 2 * n + grp;
+          ok = __all_sync(0xffffffffu, mbar_wait(&s_full[grp], sc & 1));
+          if (ok && lane == 0) mbar_arrive(s_free);
+          if (ok && sc > 0) ok = __all_sync(0xffffffffu, mbar_wait(&p_done[grp], (sc - 1) & 1));
+          ok = ok && zero_pads(j, (d.t0 + j) * kChTile);
+          __syncwarp();
+          if (ok && lane == 0) {
+            mbar_arrive(&p_half[grp]);
+            mbar_arrive(&p_full[grp]);
+          }
+        }
+      }
+      for (int n = 0; n < n_mine && !idle; ++n) {
         const int j = dual ? n : 2 * n + grp;
         const int k0 = (d.t0 + j) * kChTile;
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[grp], sc & 1));
         if (!ok) break;
-        ++sc;
         tc_fence_after();
-        // Slots outside the block's range may hold anything: their V rows become
-        // zeros, so that 0 * V stays 0 (whole pages outside are zeros already).
-        // (DUAL: group 0 does it; group 1's product is issued after group 0's.)
-        const int z0 = min(max(d.lo - k0, 0), kChTile), z1 = min(max(d.hi - k0, 0), kChTile);
-        if ((((z0 | z1) & 15) != 0) && (!dual || grp == 0)) {
-          const unsigned s = seq0 + unsigned(chunk_vseq(j, lag, d.nt));
-          ok = __all_sync(0xffffffffu, mbar_wait(&full[s % NS], (s / NS) & 1));
-          if (!ok) break;
-          const uint32_t vb = smem_u32(tiles + G::kRingOff) + uint32_t(s % NS) * G::kRowTile;
-          const int pad0 = z0 & 15, pad1 = (16 - (z1 & 15)) & 15;
-          for (int c = row; c < (pad0 + pad1) * KB * 8; c += 128) {
-            const int i = c / (KB * 8), rem = c % (KB * 8);
-            const int key = i < pad0 ? z0 - 1 - i : z1 + (i - pad0);
-            st_shared_v4(vb + (key >> 3) * G::kGroupBytes + (rem >> 3) * 1024 + (key & 7) * 128 +
-                             ((rem & 7) << 4), 0u, 0u, 0u, 0u);
-          }
-          fence_proxy_async_smem();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, s[c]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_bind32(s[c]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free);
+        // Scores in log2 units when they are capped or biased; otherwise the
+        // scale (> 0) waits for the exponent's multiply-add.
+        if constexpr (MOD != 0) {
+          const float d0 = float(k0 - pos);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              float x = __uint_as_float(s[c][e]);
+              if constexpr (MOD & 1)  // cap * tanh(u) = cap - 2 cap / (1 + exp(2 u))
+                x = fmaf(-2.f * p.cap_log2, fast_rcp(1.f + fast_exp2(x * p.cap_arg)), p.cap_log2);
+              else
+                x *= p.scale_log2;
+              if constexpr (MOD & 2) x = fmaf(-slope, fabsf(d0 + float(c * 32 + e)), x);
+              s[c][e] = __float_as_uint(x);
+            }
         }
-        if (!idle) {
-          uint32_t s[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, s[c]);
-          tmem_ld_wait();
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_bind32(s[c]);
-          // Scores in log2 units when they are capped or biased; otherwise the
-          // scale (> 0) waits for the exponent's multiply-add.
-          if constexpr (MOD != 0) {
-            const float d0 = float(k0 - pos);
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                float x = __uint_as_float(s[c][e]);
-                if constexpr (MOD & 1)  // cap * tanh(u) = cap - 2 cap / (1 + exp(2 u))
-                  x = fmaf(-2.f * p.cap_log2, fast_rcp(1.f + fast_exp2(x * p.cap_arg)), p.cap_log2);
-                else
-                  x *= p.scale_log2;
-                if constexpr (MOD & 2) x = fmaf(-slope, fabsf(d0 + float(c * 32 + e)), x);
-                s[c][e] = __float_as_uint(x);
-              }
-          }
-          const int a = lo - k0, b = hi - k0;
-          if (!__all_sync(0xffffffffu, a <= 0 && b >= kChTile)) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int bc = min(max(b - c * 32, 0), 32), ac = min(max(a - c * 32, 0), 32);
-              const uint32_t below_b = bc == 32 ? 0xffffffffu : (1u << bc) - 1u;
-              const uint32_t below_a = ac == 32 ? 0xffffffffu : (1u << ac) - 1u;
-              const uint32_t bits = below_b & ~below_a;
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!((bits >> e) & 1u)) s[c][e] = __float_as_uint(kNegInf);
-            }
-          }
-          float mx;
-          {
-            float m8[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              m8[i] = fmax3(__uint_as_float(s[0][i]), __uint_as_float(s[0][i + 8]),
-                            __uint_as_float(s[0][i + 16]));
-              m8[i] = fmax3(m8[i], __uint_as_float(s[0][i + 24]), __uint_as_float(s[1][i]));
-#pragma unroll
-              for (int q = 1; q < 4; ++q) {
-                m8[i] = fmax3(m8[i], __uint_as_float(s[q][i + 8]), __uint_as_float(s[q][i + 16]));
-                if (q < 3)
-                  m8[i] = fmax3(m8[i], __uint_as_float(s[q][i + 24]), __uint_as_float(s[q + 1][i]));
-                else
-                  m8[i] = fmaxf(m8[i], __uint_as_float(s[q][i + 24]));
-              }
-            }
-            mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
-          }
-          if constexpr (MOD == 0) mx *= p.scale_log2;  // -inf stays -inf
-          // Lazy maximum: the reference moves only when a row's maximum grows by
-          // more than 2^8, with probabilities up to 2^8 until then.
-          float alpha = 1.f;
-          bool rescale = false;
-          if (mx > m_ref + 8.f) {
-            alpha = fast_exp2(m_ref - mx);
-            rescale = m_ref != kNegInf;
-            m_ref = mx;
-            l_sum *= alpha;
-          }
-          const float mb = m_ref == kNegInf ? 0.f : -m_ref;
-          float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
+        const int a = lo - k0, b = hi - k0;
+        const bool open = __all_sync(0xffffffffu, a <= 0 && b >= kChTile);  // no mask
+        if (!open) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t ph[16];
+            const int bc = min(max(b - c * 32, 0), 32), ac = min(max(a - c * 32, 0), 32);
+            const uint32_t below_b = bc == 32 ? 0xffffffffu : (1u << bc) - 1u;
+            const uint32_t below_a = ac == 32 ? 0xffffffffu : (1u << ac) - 1u;
+            const uint32_t bits = below_b & ~below_a;
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              float x0, x1, x2, x3;
-              fma_pair(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]),
-                       MOD ? 1.f : p.scale_log2, mb, x0, x1);
-              fma_pair(__uint_as_float(s[c][e + 2]), __uint_as_float(s[c][e + 3]),
-                       MOD ? 1.f : p.scale_log2, mb, x2, x3);
-              x0 = fast_exp2(x0);
-              x1 = fast_exp2(x1);
-              x2 = fast_exp2(x2);
-              x3 = fast_exp2(x3);
-              add_pair(l0, l1, x0, x1);
-              add_pair(l2, l3, x2, x3);
-              // (P in the input's 16 bits: one rounding of half a step a term, the
-              // A operand's type; the sum l keeps the unrounded values)
-              ph[e / 2] = pack_pair<T>(x0, x1);
-              ph[e / 2 + 1] = pack_pair<T>(x2, x3);
-            }
-            tmem_st16(tS + c * 16, ph);
+            for (int e = 0; e < 32; ++e)
+              if (!((bits >> e) & 1u)) s[c][e] = __float_as_uint(kNegInf);
           }
-          l_sum += (l0 + l1) + (l2 + l3);
-          // O moves to the new reference. Its last product is complete: this
-          // tile's S was issued after it and has been waited for.
-          if (__any_sync(0xffffffffu, rescale)) {
+        }
+        float mx;
+        {
+          float m8[8];
 #pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(tO + c, o);
-              tmem_ld_wait();
-              tmem_bind32(o);
+          for (int i = 0; i < 8; ++i) {
+            m8[i] = fmax3(__uint_as_float(s[0][i]), __uint_as_float(s[0][i + 8]),
+                          __uint_as_float(s[0][i + 16]));
+            m8[i] = fmax3(m8[i], __uint_as_float(s[0][i + 24]), __uint_as_float(s[1][i]));
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_st32(tO + c, o);
+            for (int q = 1; q < 4; ++q) {
+              m8[i] = fmax3(m8[i], __uint_as_float(s[q][i + 8]), __uint_as_float(s[q][i + 16]));
+              if (q < 3)
+                m8[i] = fmax3(m8[i], __uint_as_float(s[q][i + 24]), __uint_as_float(s[q + 1][i]));
+              else
+                m8[i] = fmaxf(m8[i], __uint_as_float(s[q][i + 24]));
             }
+          }
+          mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
+        }
+        if constexpr (MOD == 0) mx *= p.scale_log2;  // -inf stays -inf
+        // P of the last tile has been read, and O holds its product.
+        if (sc > 0) ok = __all_sync(0xffffffffu, mbar_wait(&p_done[grp], (sc - 1) & 1));
+        ok = ok && zero_pads(j, k0);
+        if (!ok) break;
+        ++sc;
+        tc_fence_after();
+        // Lazy maximum: the reference moves only when a row's maximum grows by
+        // more than 2^8, with probabilities up to 2^8 until then.
+        float alpha = 1.f;
+        bool rescale = false;
+        if (mx > m_ref + 8.f) {
+          alpha = fast_exp2(m_ref - mx);
+          rescale = m_ref != kNegInf;
+          m_ref = mx;
+          l_sum *= alpha;
+        }
+        // O moves to the new reference (rare; eight columns at a time, the scores
+        // being in registers).
+        if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 8) {
+            uint32_t o[8];
+            tmem_ld8(tO + c, o);
+            tmem_ld_wait();
+            tmem_bind8(o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st8(tO + c, o);
           }
           tmem_st_wait();
         }
+        const float mb = m_ref == kNegInf ? 0.f : -m_ref;
+        float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t ph[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            float x0, x1, x2, x3;
+            fma_pair(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]),
+                     MOD ? 1.f : p.scale_log2, mb, x0, x1);
+            fma_pair(__uint_as_float(s[c][e + 2]), __uint_as_float(s[c][e + 3]),
+                     MOD ? 1.f : p.scale_log2, mb, x2, x3);
+            x0 = fast_exp2(x0);
+            x1 = fast_exp2(x1);
+            x2 = fast_exp2(x2);
+            x3 = fast_exp2(x3);
+            add_pair(l0, l1, x0, x1);
+            add_pair(l2, l3, x2, x3);
+            // (P in the input's 16 bits: one rounding of half a step a term, the A
+            // operand's type; the sum l keeps the unrounded values)
+            ph[e / 2] = pack_pair<T>(x0, x1);
+            ph[e / 2 + 1] = pack_pair<T>(x2, x3);
+          }
+          tmem_st16(tP + c * 16, ph);
+          if (c == 1) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_half[grp]);
+          }
+        }
+        l_sum += (l0 + l1) + (l2 + l3);
+        tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[grp]);
       }
       if (!ok) break;
-      seq0 += 2u * unsigned(d.nt);
+      tile0 += unsigned(d.nt);
 
       // -------------------------------------------------------------- epilogue
-      ok = __all_sync(0xffffffffu, mbar_wait(&o_full[grp], k & 1) &&
-                                       (dual || mbar_wait(&o_full[grp ^ 1], k & 1)));
+      if (sc > 0) ok = __all_sync(0xffffffffu, mbar_wait(&p_done[grp], (sc - 1) & 1));
       if (!ok) break;
       tc_fence_after();
       // The row's factor on each group's O (0 where it saw no key), its columns
@@ -840,11 +927,14 @@ __global__ void __launch_bounds__(kChThreads, 1)
       float f0, f1 = 0.f, m_out = m_ref, l_out = l_sum;
       int c0 = 0, c1 = D;
       if (!dual) {
+        // (the other group's (m, l) come once its products are complete too)
         ml_x[grp * 128 + row] = make_float2(m_ref, l_sum);
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&xch[grp]);
         ok = __all_sync(0xffffffffu, mbar_wait(&xch[grp ^ 1], alt & 1));
         if (!ok) break;
+        tc_fence_after();
         const float2 a = ml_x[row], b = ml_x[128 + row];
         m_out = fmaxf(a.x, b.x);
         f0 = a.x == kNegInf ? 0.f : fast_exp2(a.x - m_out);
@@ -895,11 +985,14 @@ __global__ void __launch_bounds__(kChThreads, 1)
               for (int e = 0; e < 32; e += 4)
                 to[e / 4] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
             } else {
-              uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at);
+              // (a thread's row lies apart from its neighbours': whole 32-byte sectors)
+              T* to = static_cast<T*>(p.out) + at;
 #pragma unroll
-              for (int e = 0; e < 32; e += 8)
-                to[e / 8] = make_uint4(pack_pair<T>(v[e], v[e + 1]), pack_pair<T>(v[e + 2], v[e + 3]),
-                                       pack_pair<T>(v[e + 4], v[e + 5]), pack_pair<T>(v[e + 6], v[e + 7]));
+              for (int e = 0; e < 32; e += 16)
+                st_global_v8(to + e, pack_pair<T>(v[e], v[e + 1]), pack_pair<T>(v[e + 2], v[e + 3]),
+                             pack_pair<T>(v[e + 4], v[e + 5]), pack_pair<T>(v[e + 6], v[e + 7]),
+                             pack_pair<T>(v[e + 8], v[e + 9]), pack_pair<T>(v[e + 10], v[e + 11]),
+                             pack_pair<T>(v[e + 12], v[e + 13]), pack_pair<T>(v[e + 14], v[e + 15]));
             }
           }
           __syncwarp();
@@ -915,6 +1008,8 @@ __global__ void __launch_bounds__(kChThreads, 1)
         ++alt;
         tc_fence_after();
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&desc_empty[ds]);
     }
     if (!ok && lane == 0) atomicOr(p.err, kErrTimeout);
     tc_fence_before();

@@ -30,7 +30,7 @@
 
 static_assert(bc::kCowPlanMaxNodes == BC_MAX_NODES, "the planner's node cap is the API's");
 static_assert(bc::kAppendMaxBatch == BC_MAX_SEQUENCES && bc::kBeamMax == BC_MAX_BEAMS &&
-                  bc::kBeamMaxVocab == BC_MAX_BEAM_VOCAB,
+                  bc::kBeamMaxVocab == BC_MAX_BEAM_VOCAB && bc::kChMaxBatch == BC_MAX_CHUNK_REQUESTS,
               "the kernels' limits are the API's");
 
 namespace bc {
@@ -1298,7 +1298,8 @@ int bc_chunk_attention(const bc_shape* s, int tokens, int dtype, const void* q,
                        int output_f32, void* workspace, size_t workspace_bytes, void* stream) {
   if (!chunk_shape_ok(s) || tokens < 0 || (dtype != BC_F16 && dtype != BC_BF16) || !q || !k ||
       !v || !layout_ok(layout, s->physical_pages) || layout->head_stride % 64 || !pages ||
-      !query_start || !lengths || !options || !output || (address_bits(q, k, v, output) % 16) ||
+      !query_start || !lengths || !options || !output || (address_bits(q, k, v) % 16) ||
+      address_bits(output) % 32 ||
       (q_stride & 7) || q_stride < 0 || !(options->scale > 0.f) || std::isinf(options->scale) ||
       !(options->softcap >= 0.f) || std::isinf(options->softcap) || options->window < 0)
     return cudaErrorInvalidValue;

@@ -404,9 +404,11 @@ typedef struct bc_chunk_options {
  * request sees must be finite. Malformed starts and lengths are brought into
  * range and set BC_ERR_LENGTH; a seen page outside the pool reads as zeros and
  * sets BC_ERR_PAGE_RANGE. query_heads / kv_heads at most 128; addresses and
- * strides are multiples of 16 bytes, head_stride one of 64 elements.
+ * strides are multiples of 16 bytes, output's of 32, head_stride one of 64
+ * elements; batch at most BC_MAX_CHUNK_REQUESTS.
  * workspace: bc_chunk_workspace_bytes, 16-byte aligned, one per call in
  * flight (0 bytes: may be NULL). */
+#define BC_MAX_CHUNK_REQUESTS 16384
 size_t bc_chunk_workspace_bytes(const bc_shape* shape, int tokens);
 int bc_chunk_attention(const bc_shape* shape, int tokens, int dtype, const void* q,
                        long long q_stride, const void* k, const void* v,
