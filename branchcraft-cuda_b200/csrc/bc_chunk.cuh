@@ -43,9 +43,11 @@ namespace bc {
 constexpr int kChThreads = 384;
 constexpr int kChTile = 128;      // keys of a tile: eight pages
 constexpr int kChDescs = 4;       // item descriptors in flight
-constexpr int kChMaxBatch = 16384;
+constexpr int kChMaxBatch = 4096;
 constexpr int kChMinPiece = 4;    // key tiles: the granularity of cuts inside an item
-constexpr int kChItemCost = 3;    // what an item costs beside its key tiles, in key tiles
+// What the shares balance, in the time of an ALT key tile: a DUAL tile is two, and
+// an item costs this much beside its tiles (its Q, its first scores, its epilogue).
+constexpr int kChItemCost = 5;
 // Registers: launched at 168 a thread (65,536 / 384, in eights); the softmax
 // groups grow to 208 (a row's 128 scores stay in registers), the others shrink
 // to 88: together the launch's total.
@@ -68,7 +70,7 @@ struct ChunkParams {
   void* out;                  // [tokens, hq, D]
   int out_f32;
   float scale_log2;           // scale * log2(e)
-  float cap_log2, cap_arg;    // softcap * log2(e), 2 log2(e) scale / softcap
+  float cap_log2, cap_u;      // softcap * log2(e), scale / softcap
   // workspace of split items (null when none can be split)
   float4* part_o;             // [blocks * 2][D / 4][part_rows]
   float2* part_ml;            // [blocks * 2][part_rows]
@@ -118,6 +120,15 @@ __device__ __forceinline__ ChunkRange chunk_range(const ChunkParams& p, const Ch
   return g;
 }
 
+// A block's share of the work: its number of key tiles times this, and kChItemCost.
+__device__ __forceinline__ int chunk_weight(const ChunkParams& p, int cnt) {
+  return cnt > p.tile_tokens ? 2 : 1;
+}
+__device__ __forceinline__ int chunk_cost(const ChunkParams& p, const ChunkRequest& r, int blk) {
+  const int i0 = blk * 2 * p.tile_tokens, cnt = min(2 * p.tile_tokens, r.n - i0);
+  return kChItemCost + chunk_weight(p, cnt) * chunk_range(p, r, i0, cnt).tiles;
+}
+
 // One piece of an item, as every role reads it.
 struct ChunkDesc {
   int first, ntok;       // the block's first token (row of q) and its tokens
@@ -147,7 +158,7 @@ struct ChunkGeom {
   static constexpr int kMlOff = kRingOff + kStages * kRowTile;  // [2][128] (m, l)
   static constexpr int kTileBytes = kMlOff + 2 * 128 * 8;
   static_assert(kMiscBytes <= 1008, "the small state fits before the first tile");
-  static_assert(kChMaxBatch * 8 <= kStages * kRowTile, "the plan's sums fit in the ring");
+  static_assert(kChMaxBatch * 24 <= kStages * kRowTile, "the plan's requests fit in the ring");
   // with `fixed` bytes of static shared memory before the dynamic part
   static size_t smem_bytes(size_t fixed) {
     const size_t at = (fixed + 15) / 16 * 16;
@@ -235,6 +246,28 @@ __device__ __forceinline__ void add_pair(float& a0, float& a1, float b0, float b
       "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
       : "+f"(a0), "+f"(a1)
       : "f"(b0), "f"(b1));
+}
+
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// Largest magnitude of three.
+__device__ __forceinline__ float fmax3_abs(float a, float b, float c) {
+  float r;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // 32 bytes at once (the address a multiple of 32).
@@ -344,9 +377,10 @@ __global__ void __launch_bounds__(kChThreads, 1)
   grid_launch_dependents();  // (TMEM is allocated: a waiting successor cannot hold it back)
   grid_dependency_wait();
 
-  // ---- plan: the cost of every request (per KV head), into the idle ring
+  // ---- plan: every request and its cost (per KV head), into the idle rings
   const int block_tokens = 2 * p.tile_tokens;
-  long long* tot = reinterpret_cast<long long*>(tiles + G::kRingOff);
+  long long* cost_of = reinterpret_cast<long long*>(tiles + G::kRingOff);
+  ChunkRequest* request_of = reinterpret_cast<ChunkRequest*>(cost_of + kChMaxBatch);
   for (int base = warp * 32; base < p.batch; base += (kChThreads / 32) * 32) {
     const int b = base + lane;
     ChunkRequest r = {0, 0, 0, 0};
@@ -354,9 +388,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
     const int nblk = (r.n + block_tokens - 1) / block_tokens;
     long long sum = 0;
     if (nblk <= 4)
-      for (int j = 0; j < nblk; ++j)
-        sum += kChItemCost +
-               chunk_range(p, r, j * block_tokens, min(block_tokens, r.n - j * block_tokens)).tiles;
+      for (int j = 0; j < nblk; ++j) sum += chunk_cost(p, r, j);
     for (unsigned many = __ballot_sync(0xffffffffu, nblk > 4); many; many &= many - 1) {
       const int src = __ffs(many) - 1;  // a long chunk: its blocks spread over the warp
       const ChunkRequest o = {__shfl_sync(0xffffffffu, r.first, src),
@@ -364,13 +396,15 @@ __global__ void __launch_bounds__(kChThreads, 1)
                               __shfl_sync(0xffffffffu, r.len, src),
                               __shfl_sync(0xffffffffu, r.prefix, src)};
       long long part = 0;
-      for (int i0 = lane * block_tokens; i0 < o.n; i0 += 32 * block_tokens)
-        part += kChItemCost + chunk_range(p, o, i0, min(block_tokens, o.n - i0)).tiles;
+      for (int j = lane; j * block_tokens < o.n; j += 32) part += chunk_cost(p, o, j);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
       if (lane == src) sum = part;
     }
-    if (b < p.batch) tot[b] = sum;
+    if (b < p.batch) {
+      cost_of[b] = sum;
+      request_of[b] = r;
+    }
   }
   fence_proxy_async_smem();  // (copies will follow into the same memory)
   __syncthreads();
@@ -381,82 +415,103 @@ __global__ void __launch_bounds__(kChThreads, 1)
     regs_decrease<kChOtherRegs>();
     if (warp == 8) {
       // ---------------------------------------------------------- scheduler
-      const int per_lane = (p.batch + 31) / 32;
-      const int sb0 = min(p.batch, lane * per_lane), sb1 = min(p.batch, sb0 + per_lane);
-      long long mine = 0;
-      for (int b = sb0; b < sb1; ++b) mine += tot[b];
-      long long incl = mine;
+      // This block's share: from its own cut (found by lanes 0-15) up to the next
+      // block's (lanes 16-31). Cuts inside an item fall on multiples of `grain`
+      // tiles from its start (a thirty-second of a share, at least kChMinPiece: a
+      // piece costs its partial state's way through memory) or on its ends.
+      const int half = lane >> 4, hl = lane & 15;
+      const int per_lane = (p.batch + 15) / 16;
+      const int sb0 = min(p.batch, hl * per_lane), sb1 = min(p.batch, sb0 + per_lane);
+      auto scan = [&](long long v) {  // inclusive, over the lanes of a half
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += up;
-      }
-      const long long cost = __shfl_sync(0xffffffffu, incl, 31) * p.hkv;  // of the whole call
-      const long long pre = incl - mine;
-      // Cuts inside an item fall on multiples of `grain` tiles from its start (a
-      // thirty-second of a share, at least kChMinPiece: a piece costs its partial
-      // state's way through memory) or on its ends.
-      const long long share = cost / gridDim.x;
-      const int grain = int(max((long long)kChMinPiece, min(share / 32, 1ll << 20)));
-      // A place in the sequence of key tiles: tile `off` of an item.
+        for (int d = 1; d < 16; d <<= 1) {
+          const long long up = __shfl_up_sync(0xffffffffu, v, d, 16);
+          if (hl >= d) v += up;
+        }
+        return v;
+      };
+      // the half's last lane whose run (of cost `mine` per head, after `pre`) begins
+      // at or before u
+      auto owner = [&](long long mine, long long pre, long long u) -> int {
+        const unsigned at =
+            (__ballot_sync(0xffffffffu, mine > 0 && pre * p.hkv <= u) >> (16 * half)) & 0xffffu;
+        return at ? 31 - __clz(at) : 0;
+      };
+      long long mine = 0;
+      for (int b = sb0; b < sb1; ++b) mine += cost_of[b];
+      long long incl = scan(mine);
+      const long long cost = __shfl_sync(0xffffffffu, incl, 15, 16) * p.hkv;  // of the whole call
+      const long long u = (long long)(double(cost) * double(blockIdx.x + half) / double(gridDim.x));
+      const bool in = u < cost;  // (else the call's end: request p.batch)
+      // the request
       int req = p.batch, blk = 0, head = 0, off = 0;
+      long long at = incl - mine;
+      int src = owner(mine, at, u);
+      if (in && hl == src)
+        for (req = sb0; (at + cost_of[req]) * p.hkv <= u; ++req) at += cost_of[req];
+      req = __shfl_sync(0xffffffffu, req, src, 16);
+      long long rem = u - __shfl_sync(0xffffffffu, at, src, 16) * p.hkv;
       ChunkRequest r = {0, 0, 0, 0};
+      if (in) r = request_of[req];
+      // its block, a run of consecutive ones a lane
+      const int nblk = (r.n + block_tokens - 1) / block_tokens;
+      const int run = (nblk + 15) / 16, j0 = min(nblk, hl * run), j1 = min(nblk, j0 + run);
+      mine = 0;
+      for (int j = j0; j < j1; ++j) mine += chunk_cost(p, r, j);
+      incl = scan(mine);
+      at = incl - mine;
+      src = owner(mine, at, rem);
+      int n = 1;
+      if (in && hl == src)
+        for (blk = j0; n = chunk_cost(p, r, blk), (at + n) * p.hkv <= rem; ++blk) at += n;
+      blk = __shfl_sync(0xffffffffu, blk, src, 16);
+      n = __shfl_sync(0xffffffffu, n, src, 16);
+      rem -= __shfl_sync(0xffffffffu, at, src, 16) * p.hkv;
+      // its head and tile
+      const int weight = chunk_weight(p, r.n - blk * block_tokens);
+      const int grain = max(kChMinPiece, int(min(cost / gridDim.x / (32 * weight), 1ll << 20)));
+      if (in) {
+        head = int(double(rem) / double(n));
+        off = max(int(rem - (long long)head * n) - kChItemCost, 0) / weight;
+        n = (n - kChItemCost) / weight;
+        off = (off + grain / 2) / grain * grain;
+        if (off > 0 && n - off < (grain + 1) / 2) {  // the next item's start
+          off = 0;
+          if (++head == p.hkv) {
+            head = 0;
+            if (++blk == nblk) {
+              blk = 0;
+              do {
+                ++req;
+              } while (req < p.batch && request_of[req].n == 0);
+              if (req < p.batch) r = request_of[req];
+            }
+          }
+        }
+      }
+      const int e_req = __shfl_sync(0xffffffffu, req, 16), e_blk = __shfl_sync(0xffffffffu, blk, 16),
+                e_head = __shfl_sync(0xffffffffu, head, 16), e_off = __shfl_sync(0xffffffffu, off, 16);
+      req = __shfl_sync(0xffffffffu, req, 0);
+      blk = __shfl_sync(0xffffffffu, blk, 0);
+      head = __shfl_sync(0xffffffffu, head, 0);
+      off = __shfl_sync(0xffffffffu, off, 0);
+      r.first = __shfl_sync(0xffffffffu, r.first, 0);
+      r.n = __shfl_sync(0xffffffffu, r.n, 0);
+      r.len = __shfl_sync(0xffffffffu, r.len, 0);
+      r.prefix = __shfl_sync(0xffffffffu, r.prefix, 0);
       ChunkRange g = {0, 0, 0, 1};
       auto load_block = [&] {  // the current block's range
-        g = chunk_range(p, r, blk * block_tokens,
-                        min(block_tokens, r.n - blk * block_tokens));
+        g = chunk_range(p, r, blk * block_tokens, min(block_tokens, r.n - blk * block_tokens));
       };
-      auto cut = [&](long long u) {  // the place of cost u (the call's end: request p.batch)
-        off = head = blk = 0;
-        req = p.batch;
-        if (u >= cost) return;
-        const unsigned below = __ballot_sync(0xffffffffu, mine > 0 && pre * p.hkv <= u);
-        const int src = 31 - __clz(below);
-        int found = 0;
-        long long at = pre;
-        if (lane == src)
-          for (found = sb0; (at + tot[found]) * p.hkv <= u; ++found) at += tot[found];
-        req = __shfl_sync(0xffffffffu, found, src);
-        long long rem = u - __shfl_sync(0xffffffffu, at, src) * p.hkv;
-        r = chunk_request(p, req);
-        const int nblk = (r.n + block_tokens - 1) / block_tokens;
-        int n = 1;
-        for (int j0 = 0;; j0 += 32) {  // the block among the request's
-          const int j = j0 + lane;
-          const int t = j < nblk ? kChItemCost + chunk_range(p, r, j * block_tokens,
-                                                             min(block_tokens, r.n - j * block_tokens)).tiles
-                                 : 0;
-          long long in = t;
-#pragma unroll
-          for (int d = 1; d < 32; d <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, in, d);
-            if (lane >= d) in += up;
-          }
-          const unsigned after = __ballot_sync(0xffffffffu, in * p.hkv > rem);
-          if (after) {
-            const int w = __ffs(after) - 1;
-            blk = j0 + w;
-            n = __shfl_sync(0xffffffffu, t, w);
-            rem -= (__shfl_sync(0xffffffffu, in, w) - n) * p.hkv;
-            break;
-          }
-          rem -= __shfl_sync(0xffffffffu, in, 31) * p.hkv;
-        }
-        head = int(rem / n);
-        off = max(int(rem % n) - kChItemCost, 0);
-        n -= kChItemCost;
-        off = (off + grain / 2) / grain * grain;
-        if (off > 0 && n - off < (grain + 1) / 2) off = n;
-        load_block();
-      };
+      if (req < p.batch) load_block();
       auto next_item = [&] {
         off = 0;
         if (++head < p.hkv) return;
         head = 0;
         if ((++blk) * block_tokens >= r.n) {
           blk = 0;
-          // the next request with tokens (the sums of the plan are gone: the
-          // ring is in use), 32 looked at together
+          // the next request with tokens (the plan is gone: the rings are in use),
+          // 32 looked at together
           for (++req; req < p.batch; req += 32) {
             const int b = req + lane;
             const bool some = b < p.batch && chunk_request(p, b).n > 0;
@@ -471,12 +526,6 @@ __global__ void __launch_bounds__(kChThreads, 1)
         }
         if (req < p.batch) load_block();
       };
-      // This block's share: from its own cut up to the next block's.
-      cut(cost * (blockIdx.x + 1) / gridDim.x);
-      if (req < p.batch && off >= g.tiles) next_item();
-      const int e_req = req, e_blk = blk, e_head = head, e_off = off;
-      cut(cost * blockIdx.x / gridDim.x);
-      if (req < p.batch && off >= g.tiles) next_item();
       // tiles of the current item that are this block's, from `off` on
       auto mine_here = [&]() -> int {
         if (req >= p.batch) return 0;
@@ -798,19 +847,56 @@ __global__ void __launch_bounds__(kChThreads, 1)
         if (lane == 0) mbar_arrive(s_free);
         // Scores in log2 units when they are capped or biased; otherwise the
         // scale (> 0) waits for the exponent's multiply-add.
-        if constexpr (MOD != 0) {
+        if constexpr (MOD & 1) {
+          // cap * tanh(u), u = x scale / cap. While the warp's |u| stay below 3/4, as
+          // scores of a model trained with its cap do, by the polynomial
+          // v + v t P(t), v = x scale log2(e), t = u^2, P of degree 4 with the least
+          // largest error of tanh on [0, 3/4] (1.3e-8, fitted for this kernel): two
+          // scores an instruction. Else cap - 2 cap / (1 + exp(2 u)), two more
+          // results of the exponential unit a score, which bounds the softmax.
+          float big = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+              big = fmax3_abs(big, __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+          if (__all_sync(0xffffffffu, big * p.cap_u < 0.75f)) {
+            const uint64_t arg = pair_of(p.cap_u, p.cap_u), sl = pair_of(p.scale_log2, p.scale_log2);
+            const uint64_t c1 = pair_of(-0.33332908153533936f, -0.33332908153533936f),
+                           c2 = pair_of(0.13324248790740967f, 0.13324248790740967f),
+                           c3 = pair_of(-0.05328230932354927f, -0.05328230932354927f),
+                           c4 = pair_of(0.01945533975958824f, 0.01945533975958824f),
+                           c5 = pair_of(-0.004626113455742598f, -0.004626113455742598f);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const uint64_t x = pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+                const uint64_t u = mul2(x, arg), t = mul2(u, u), v = mul2(x, sl);
+                const uint64_t P = fma2(t, fma2(t, fma2(t, fma2(t, c5, c4), c3), c2), c1);
+                const uint64_t y = fma2(v, mul2(t, P), v);
+                asm("mov.b64 {%0, %1}, %2;" : "=r"(s[c][e]), "=r"(s[c][e + 1]) : "l"(y));
+              }
+          } else {
+            const float arg = 2.f * 1.4426950408889634f * p.cap_u;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                s[c][e] = __float_as_uint(fmaf(
+                    -2.f * p.cap_log2, fast_rcp(1.f + fast_exp2(__uint_as_float(s[c][e]) * arg)),
+                    p.cap_log2));
+          }
+        }
+        if constexpr (MOD & 2) {
           const float d0 = float(k0 - pos);
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
-              float x = __uint_as_float(s[c][e]);
-              if constexpr (MOD & 1)  // cap * tanh(u) = cap - 2 cap / (1 + exp(2 u))
-                x = fmaf(-2.f * p.cap_log2, fast_rcp(1.f + fast_exp2(x * p.cap_arg)), p.cap_log2);
-              else
-                x *= p.scale_log2;
-              if constexpr (MOD & 2) x = fmaf(-slope, fabsf(d0 + float(c * 32 + e)), x);
-              s[c][e] = __float_as_uint(x);
+              const float x = __uint_as_float(s[c][e]);
+              s[c][e] = __float_as_uint(fmaf(-slope, fabsf(d0 + float(c * 32 + e)),
+                                             (MOD & 1) ? x : x * p.scale_log2));
             }
         }
         const int a = lo - k0, b = hi - k0;
@@ -1033,29 +1119,40 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkParams p) {
   const int tok = (row / 128) * p.tile_tokens + (row % 128) / p.group;
   const bool valid = row < p.part_rows && (row % 128) / p.group < p.tile_tokens && tok < ntok;
   if (!__any_sync(0xffffffffu, valid)) return;
-  int end = c + 1;  // one past the block that ends the item
-  while (end < blocks && p.sched[size_t(end) * 8] != 2) ++end;
-  end = min(end + 1, blocks);
-  auto none = [&](int i) { return i != c && p.sched[size_t(i) * 8] == 3; };
-  auto slot = [&](int i) -> size_t { return i == c ? size_t(c) * 2 + 1 : size_t(i) * 2; };
+  // Where the pieces lie, 32 blocks looked at together: those after c that have a
+  // share, up to the one that ends the item.
+  constexpr int kMost = 160;  // (a block per SM)
+  __shared__ int s_slot[4][kMost];
+  int* slot = s_slot[warp];
+  int n = 1;
+  if (lane == 0) slot[0] = c * 2 + 1;
+  for (int i0 = c + 1;; i0 += 32) {
+    const int state = i0 + lane < blocks ? p.sched[size_t(i0 + lane) * 8] : 2;
+    const unsigned ends = __ballot_sync(0xffffffffu, state == 2);
+    const unsigned upto = ends ? ends ^ (ends - 1) : 0xffffffffu;  // through the first end
+    const unsigned has = __ballot_sync(0xffffffffu, state != 3 && i0 + lane < blocks) & upto;
+    const int at = n + __popc(has & ((1u << lane) - 1));
+    if ((has >> lane & 1) && at < kMost) slot[at] = (i0 + lane) * 2;
+    n = min(n + __popc(has), kMost);
+    if (ends) break;
+  }
+  __syncwarp();
+  if (!valid) return;
   float m = -INFINITY, l = 0.f;
-  if (valid)
-    for (int i = c; i < end; ++i)
-      if (!none(i)) m = fmaxf(m, p.part_ml[slot(i) * p.part_rows + row].x);
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) m = fmaxf(m, p.part_ml[size_t(slot[i]) * p.part_rows + row].x);
   constexpr int N = D / 16;  // float4 pieces of a warp
   float4 acc[N];
 #pragma unroll
   for (int q = 0; q < N; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (!valid) return;
-  for (int i = c; i < end; ++i) {
-    if (none(i)) continue;
-    const float2 ml = p.part_ml[slot(i) * p.part_rows + row];
-    if (ml.x == -INFINITY) continue;
-    const float w = fast_exp2(ml.x - m);
+#pragma unroll 2
+  for (int i = 0; i < n; ++i) {
+    const float2 ml = p.part_ml[size_t(slot[i]) * p.part_rows + row];
+    const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - m);  // (O of such a piece is 0)
     l += w * ml.y;
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      const float4 o = p.part_o[(slot(i) * (D / 4) + warp * N + q) * p.part_rows + row];
+      const float4 o = p.part_o[(size_t(slot[i]) * (D / 4) + warp * N + q) * p.part_rows + row];
       acc[q].x += w * o.x;
       acc[q].y += w * o.y;
       acc[q].z += w * o.z;

@@ -1129,7 +1129,7 @@ struct ChunkPlan {
     const int group = s->query_heads / s->kv_heads, tile = 128 / group;
     const long long key_tiles = (s->max_pages + kChTile / kPageSize - 1) / (kChTile / kPageSize);
     const long long items = ((long long)tokens / (2 * tile) + std::min(s->batch, tokens)) * s->kv_heads;
-    blocks = int(std::min<long long>(dev < 0 ? 148 : sm_count(dev), items * key_tiles));
+    blocks = int(std::min<long long>(std::min(dev < 0 ? 148 : sm_count(dev), 160), items * key_tiles));
     rows = tokens <= tile ? (tokens * group + 31) / 32 * 32 : 256;
     // (cuts fall on multiples of kChMinPiece tiles and leave at least half of
     // that: an item of kChMinPiece + 1 tiles is never split)
@@ -1334,7 +1334,7 @@ int bc_chunk_attention(const bc_shape* s, int tokens, int dtype, const void* q,
   p.out_f32 = output_f32;
   p.scale_log2 = options->scale * kLog2e;
   p.cap_log2 = options->softcap * kLog2e;
-  p.cap_arg = options->softcap > 0.f ? 2.f * kLog2e * options->scale / options->softcap : 0.f;
+  p.cap_u = options->softcap > 0.f ? options->scale / options->softcap : 0.f;
   p.part_rows = plan.rows;
   if (plan.bytes > 0) {
     p.part_o = static_cast<float4*>(workspace);

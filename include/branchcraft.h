@@ -408,7 +408,7 @@ typedef struct bc_chunk_options {
  * elements; batch at most BC_MAX_CHUNK_REQUESTS.
  * workspace: bc_chunk_workspace_bytes, 16-byte aligned, one per call in
  * flight (0 bytes: may be NULL). */
-#define BC_MAX_CHUNK_REQUESTS 16384
+#define BC_MAX_CHUNK_REQUESTS 4096
 size_t bc_chunk_workspace_bytes(const bc_shape* shape, int tokens);
 int bc_chunk_attention(const bc_shape* shape, int tokens, int dtype, const void* q,
                        long long q_stride, const void* k, const void* v,
