@@ -160,6 +160,17 @@ def commit_batch_(cache_k, cache_v, draft_k, draft_v, clone_src, clone_dst, entr
         entry_page, entry_slot)
 
 
+# (resolved once: a packet's look-up of its overload costs a step's small calls)
+_append_plan = torch.ops.branchcraft.append_plan.default
+_append_plan_ = torch.ops.branchcraft.append_plan_.default
+_append_kv_ = torch.ops.branchcraft.append_kv_.default
+_chunk_attention = torch.ops.branchcraft.chunk_attention.default
+_chunk_attention_out = torch.ops.branchcraft.chunk_attention_out.default
+_beam_select = torch.ops.branchcraft.beam_select.default
+_beam_reorder = torch.ops.branchcraft.beam_reorder.default
+_beam_reorder_ = torch.ops.branchcraft.beam_reorder_.default
+
+
 def append_plan(pages, lengths, new_tokens, refcount, free_stack, free_count, max_tokens,
                 max_pages=0):
     """Give every sequence's new tokens their pages and slots under the pool's rules (reference
@@ -167,21 +178,21 @@ def append_plan(pages, lengths, new_tokens, refcount, free_stack, free_count, ma
     lengths, refcount, free_stack, free_count) and (query_start [S + 1], slot_map [max_tokens],
     positions [max_tokens], clones [3, S], counts [3]: tokens, clones, status). A nonzero status
     (1 bad counts, 2 pool exhausted, 3 malformed tables) plans nothing."""
-    return torch.ops.branchcraft.append_plan(pages, lengths, new_tokens, refcount, free_stack,
+    return _append_plan(pages, lengths, new_tokens, refcount, free_stack,
                                              free_count, max_tokens, max_pages)
 
 
 def append_plan_(pages, lengths, new_tokens, refcount, free_stack, free_count, max_tokens):
     """append_plan updating tables, lengths and pool state in place; returns (query_start,
     slot_map, positions, clones, counts)."""
-    return torch.ops.branchcraft.append_plan_(pages, lengths, new_tokens, refcount, free_stack,
+    return _append_plan_(pages, lengths, new_tokens, refcount, free_stack,
                                               free_count, max_tokens)
 
 
 def append_kv_(cache_k, cache_v, k, v, slot_map, clones=None, counts=None):
     """Write k, v [tokens, Hkv, D] into the slots of a plan (-1: skipped), and copy its clones'
     valid slots, in one launch. Caches [P, 16, Hkv, D], strided views included."""
-    return torch.ops.branchcraft.append_kv_(cache_k, cache_v, k, v, slot_map, clones, counts)
+    return _append_kv_(cache_k, cache_v, k, v, slot_map, clones, counts)
 
 
 def chunk_attention(q, k, v, pages, query_start, lengths, scale=None, softcap=0.0, window=0,
@@ -192,14 +203,14 @@ def chunk_attention(q, k, v, pages, query_start, lengths, scale=None, softcap=0.
     `window` keeps the last keys, `key_start` [tokens] is a token's first key (packed documents);
     `softcap` caps scores by a tanh, `alibi_slopes` [Hq] take slope * distance off. Output of q's
     type; rows of tokens in no request are unspecified (chunk_attention_out leaves them)."""
-    return torch.ops.branchcraft.chunk_attention(q, k, v, pages, query_start, lengths, scale,
+    return _chunk_attention(q, k, v, pages, query_start, lengths, scale,
                                                  softcap, window, alibi_slopes, prefix, key_start)
 
 
 def chunk_attention_out(q, k, v, pages, query_start, lengths, output, scale=None, softcap=0.0,
                         window=0, alibi_slopes=None, prefix=None, key_start=None):
     """chunk_attention into a preallocated output of q's type or FP32 (CUDA-graph safe)."""
-    return torch.ops.branchcraft.chunk_attention_out(
+    return _chunk_attention_out(
         q, k, v, pages, query_start, lengths, output, scale, softcap, window, alibi_slopes,
         prefix, key_start)
 
@@ -208,18 +219,18 @@ def beam_select(logits, scores, k):
     """The k best (beam, token) pairs of every request by scores + log_softmax(logits):
     (scores [B, k] FP32, tokens [B, k], parents [B, k]), best first, ties to the lowest
     beam * vocab + token. logits [B, beams, vocab], scores [B, beams] FP32."""
-    return torch.ops.branchcraft.beam_select(logits, scores, k)
+    return _beam_select(logits, scores, k)
 
 
 def beam_reorder(pages, lengths, parents, refcount, free_stack, free_count):
     """Page tables [B, beams, max_pages] after parents [B, new beams] (-1 drops a row): returns
     (pages, lengths, refcount, free_stack, free_count), every new row forked from its parent,
     every old one released, unheld pages pushed on the free stack."""
-    return torch.ops.branchcraft.beam_reorder(pages, lengths, parents, refcount, free_stack,
+    return _beam_reorder(pages, lengths, parents, refcount, free_stack,
                                               free_count)
 
 
 def beam_reorder_(pages, lengths, parents, refcount, free_stack, free_count):
     """beam_reorder updating the pool's state in place; returns (pages, lengths)."""
-    return torch.ops.branchcraft.beam_reorder_(pages, lengths, parents, refcount, free_stack,
+    return _beam_reorder_(pages, lengths, parents, refcount, free_stack,
                                                free_count)

@@ -1,5 +1,5 @@
 // Beam search on the device: the k best (beam, token) pairs of every request
-// (beam_chunk_kernel, beam_merge_kernel) and the page tables and reference
+// (beam_segment_kernel, beam_merge_kernel) and the page tables and reference
 // counts after the beams' new parents (beam_rows_kernel, beam_release_kernel).
 #pragma once
 
@@ -12,25 +12,27 @@ namespace bc {
 constexpr int kBeamMax = 64;      // beams of a request
 constexpr int kBeamMaxK = 64;     // pairs selected
 constexpr int kBeamMaxVocab = 1 << 20;
-constexpr int kBeamThreads = 512;
-constexpr int kBeamPerThread = 32;
-constexpr int kBeamChunk = kBeamThreads * kBeamPerThread;  // logits of one block
-constexpr int kBeamGroups = kBeamThreads / 4;              // four threads each
+constexpr int kBeamMergeThreads = 512;
+constexpr int kBeamThreads = 256;
+constexpr int kBeamPerThread = 16;
+constexpr int kBeamTile = kBeamThreads * kBeamPerThread;  // logits of one step of a block
+constexpr int kBeamGroups = kBeamThreads / 2;             // two threads each
+constexpr int kBeamKeep = 512;                            // candidates before they are thinned
+constexpr int kBeamRoom = kBeamKeep + kBeamTile;          // and the most there can be
+constexpr int kBeamThinned = kBeamMaxK * ((kBeamRoom + kBeamThreads - 1) / kBeamThreads);
 
 enum BeamType : int { kBeamF16 = 0, kBeamBF16 = 1, kBeamF32 = 2 };
 
 // A logit as the search sees it: NaN counts as -inf (never chosen before a
-// number), +inf as the largest number; -0 as +0, so that equal logits are
-// equal keys.
+// number), +inf as the largest number.
 __device__ __forceinline__ float beam_logit(float x) {
-  if (!(x > -INFINITY)) return -INFINITY;
-  return fminf(x, 3.402823466e38f) + 0.f;
+  return fminf(fmaxf(x, -INFINITY), 3.402823466e38f);
 }
 
 // Keys: larger value first, then the lower index. Unique, so selection never
-// meets a tie.
+// meets a tie. (-0 is +0: equal logits are equal in their key's value.)
 __device__ __forceinline__ unsigned beam_order(float x) {
-  const unsigned u = __float_as_uint(x);
+  const unsigned u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float beam_value(unsigned u) {
@@ -48,123 +50,243 @@ __device__ __forceinline__ double beam_value64(unsigned long long u) {
 }
 
 struct BeamSelectParams {
-  int batch, beams, vocab, k, chunks;
+  int batch, beams, vocab, k;
+  int segments, segment;  // blocks of a row, their steps' logits (a multiple of kBeamTile)
   const void* logits;
   long long row_stride;  // elements between two beams' rows
   const float* scores;   // [batch, beams]
   float* out_scores;     // [batch, k]
   int* out_tokens;
   int* out_parents;
-  // workspace, per (row, chunk): the k best keys in order (0 past the
-  // chunk's logits), the largest logit and the sum of exp(x - largest)
-  unsigned long long* keys;  // [rows, chunks, k]
-  float* chunk_max;          // [rows, chunks]
-  double* chunk_sum;         // [rows, chunks]
+  // workspace, per (row, segment): the k best keys in order (0 past the
+  // segment's logits), the largest logit and the sum of exp(x - largest)
+  unsigned long long* keys;  // [rows, segments, k]
+  float* seg_max;            // [rows, segments]
+  double* seg_sum;           // [rows, segments]
 };
 
-// One block per chunk of a row. Every thread keeps its logits in registers;
-// the threshold is the k-th largest of the 128 groups' maxima, so the chunk's
-// k best lie in k groups and a few more than k logits pass it.
 template <typename T>
-__global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(const BeamSelectParams p) {
-  __shared__ unsigned long long s_group[kBeamGroups];
-  extern __shared__ unsigned long long s_cand[];  // [k * 4 * kBeamPerThread]
+struct BeamRaw {  // a thread's logits of one step as loaded
+  static constexpr int kVec = 16 / int(sizeof(T));
+  static constexpr int kLoads = kBeamPerThread / kVec;
+  uint4 v[kLoads];
+};
+
+__device__ __forceinline__ float beam_float(const uint4& v, int i, float*) {
+  return __uint_as_float(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
+}
+__device__ __forceinline__ float beam_float(const uint4& v, int i, __half*) {
+  const uint32_t w = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
+  const float2 f = unpack_half2(w);
+  return (i & 1) ? f.y : f.x;
+}
+__device__ __forceinline__ float beam_float(const uint4& v, int i, __nv_bfloat16*) {
+  const uint32_t w = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
+  return __uint_as_float((i & 1) ? w & 0xffff0000u : w << 16);
+}
+
+// What the thinning of candidates needs beside them.
+struct BeamThin {
+  unsigned long long best[kBeamThreads];
+  unsigned long long out[kBeamMaxK];
+  unsigned long long tau;
+  int count;
+};
+
+// Keeps the k best of the n candidates in `cand` (in order, at its front), for
+// all threads of the block; returns how many there are. Many candidates are
+// thinned into `few` first: at most k threads hold keys at or above the k-th
+// largest of the threads' maxima.
+__device__ __noinline__ int beam_thin(unsigned long long* cand, unsigned long long* few, BeamThin& t,
+                                      int n, int k) {
+  const int tid = threadIdx.x;
+  const unsigned long long* from = cand;
+  if (n > 2 * kBeamThreads) {
+    unsigned long long mx = 0;
+    for (int i = tid; i < n; i += kBeamThreads) mx = cand[i] > mx ? cand[i] : mx;
+    t.best[tid] = mx;
+    if (tid == 0) t.count = 0;
+    __syncthreads();
+    int above = 0;
+#pragma unroll 8
+    for (int i = 0; i < kBeamThreads; ++i) above += t.best[i] > mx;
+    if (above == k - 1) t.tau = mx;  // (keys are unique: one thread)
+    __syncthreads();
+    if (mx >= t.tau)
+      for (int i = tid; i < n; i += kBeamThreads)
+        if (cand[i] >= t.tau) few[atomicAdd(&t.count, 1)] = cand[i];
+    __syncthreads();
+    n = t.count;
+    from = few;
+  }
+  for (int i = tid; i < n; i += kBeamThreads) {  // rank by counting
+    const unsigned long long mine = from[i];
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) above += from[j] > mine;
+    if (above < k) t.out[above] = mine;
+  }
+  __syncthreads();
+  n = min(n, k);
+  if (tid < n) cand[tid] = t.out[tid];
+  __syncthreads();
+  return n;
+}
+
+// One block per segment of a row, a step of kBeamTile logits at a time, the next
+// step's loads in flight. HBM bound: each logit is read once (16-byte loads where
+// a vector lies inside the row), compared with the k-th best so far, and added to
+// its thread's sum under the thread's own running maximum. The first step's bound
+// is the k-th largest of 128 groups' maxima (the segment's k best lie in k groups);
+// after it few logits pass, and passing ones wait in shared memory to be thinned.
+// The sum takes ex2.approx (relative error 2^-22 and that of the argument, two
+// roundings); logits that pass the bound, the ones that weigh, are put right by
+// expf, since the order of two beams' candidates hangs on the last digits; a
+// thread's 16 terms of a step are added in FP32, the steps in 64 bits.
+template <typename T>
+__global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const BeamSelectParams p) {
+  using Raw = BeamRaw<T>;
+  constexpr float kLog2E = 1.4426950408889634f;
+  constexpr int VEC = Raw::kVec;
+  extern __shared__ unsigned long long beam_cand[];  // [kBeamRoom], then [kBeamThinned]
+  __shared__ BeamThin s_thin;
   __shared__ float s_max[kBeamThreads / 32];
   __shared__ double s_sum[kBeamThreads / 32];
-  __shared__ unsigned long long s_tau;
   __shared__ int s_n;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   grid_launch_dependents();
-  grid_dependency_wait();
-  const int row = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks;
-  const int first = chunk * kBeamChunk, count = min(kBeamChunk, p.vocab - first);
-  const T* x = static_cast<const T*>(p.logits) + row * p.row_stride + first;
-  float v[kBeamPerThread];
-#pragma unroll
-  for (int j = 0; j < kBeamPerThread; ++j) {
-    const int i = j * kBeamThreads + tid;
-    v[j] = i < count ? beam_logit(float(x[i])) : -INFINITY;
-  }
-  float mx = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < kBeamPerThread; ++j) mx = fmaxf(mx, v[j]);
-  // the largest key of the thread: its first logit equal to mx
-  unsigned long long best = 0;
-#pragma unroll
-  for (int j = kBeamPerThread - 1; j >= 0; --j)
-    if (j * kBeamThreads + tid < count && v[j] == mx) best = beam_key(mx, j * kBeamThreads + tid);
-  unsigned long long g = best;
-#pragma unroll
-  for (int d = 1; d < 4; d <<= 1) {
-    const unsigned long long o = __shfl_xor_sync(0xffffffffu, g, d);
-    g = o > g ? o : g;
-  }
-  if ((lane & 3) == 0) s_group[tid >> 2] = g;
-  float wm = mx;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, d));
-  if (lane == 0) s_max[warp] = wm;
   if (tid == 0) {
     s_n = 0;
-    s_tau = 0;
+    s_thin.tau = 0;
   }
+  grid_dependency_wait();
+  const int row = blockIdx.x / p.segments, seg = blockIdx.x % p.segments;
+  const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
+  // Places count from the 16-byte boundary at or before the row: place = token + mis.
+  const int mis = int((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const T* x0 = x - mis;
+  const int w0 = seg * p.segment, w1 = min(w0 + p.segment, p.vocab + mis);
+  auto load = [&](int w, Raw& raw) {
+#pragma unroll
+    for (int j = 0; j < Raw::kLoads; ++j) {
+      const int at = w + (j * kBeamThreads + tid) * VEC;
+      if (at >= mis && at + VEC <= p.vocab + mis) {
+        raw.v[j] = __ldcs(reinterpret_cast<const uint4*>(x0 + at));
+      } else {  // a vector across the row's ends: its own logits alone
+        T e[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          e[i] = at + i >= mis && at + i < p.vocab + mis ? x0[at + i] : T(-INFINITY);
+        raw.v[j] = *reinterpret_cast<const uint4*>(e);
+      }
+    }
+  };
+  Raw raw, next;
+  if (w0 < w1) load(w0, raw);
+  float m = -INFINITY;
+  double sum = 0.0;
+  unsigned long long tau = 0;
   __syncthreads();
-  float m = s_max[0];
+  for (int w = w0; w < w1; w += kBeamTile) {
+    if (w + kBeamTile < w1) load(w + kBeamTile, next);
+    float v[kBeamPerThread];
+    float mx = -INFINITY;
 #pragma unroll
-  for (int w = 1; w < kBeamThreads / 32; ++w) m = fmaxf(m, s_max[w]);
-  // the k-th largest group maximum (empty groups are 0 and tie below it)
-  if (tid < kBeamGroups) {
-    const unsigned long long mine = s_group[tid];
-    int above = 0;
-    for (int i = 0; i < kBeamGroups; ++i) above += s_group[i] > mine;
-    if (above == p.k - 1 && mine != 0) s_tau = mine;
+    for (int j = 0; j < kBeamPerThread; ++j) {
+      v[j] = beam_logit(beam_float(raw.v[j / VEC], j % VEC, static_cast<T*>(nullptr)));
+      mx = fmaxf(mx, v[j]);
+    }
+    auto place = [&](int j) { return w + (j / VEC * kBeamThreads + tid) * VEC + j % VEC; };
+    auto key_of = [&](int j) -> unsigned long long {  // 0: no logit of the row
+      const int at = place(j);
+      return at >= mis && at < w1 ? beam_key(v[j], unsigned(at - mis)) : 0ull;
+    };
+    if (mx > m) {  // the thread's sum follows its running maximum
+      sum *= double(expf(m - mx));
+      m = mx;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    uint64_t e = 0;  // (two zeros)
+#pragma unroll
+    for (int j = 0; j < kBeamPerThread; j += 2) {
+      const float2 d = pair_floats(mul2(add2(pair_of(v[j], v[j + 1]), pair_of(-base, -base)),
+                                        pair_of(kLog2E, kLog2E)));
+      e = add2(e, pair_of(fast_exp2(d.x), fast_exp2(d.y)));
+    }
+    sum += double(pair_floats(e).x + pair_floats(e).y);
+    if (w == w0) {
+      unsigned long long best = 0;
+#pragma unroll
+      for (int j = 0; j < kBeamPerThread; ++j) {
+        const unsigned long long key = v[j] == mx ? key_of(j) : 0ull;
+        best = key > best ? key : best;
+      }
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, 1);
+      best = other > best ? other : best;
+      s_thin.best[tid] = best;
+      __syncthreads();
+      // both threads of a group count against half the groups
+      int above = 0;
+#pragma unroll 8
+      for (int i = 0; i < kBeamGroups / 2; ++i)
+        above += s_thin.best[((tid & 1) * (kBeamGroups / 2) + i) * 2] > best;
+      above += __shfl_xor_sync(0xffffffffu, above, 1);
+      if (above == p.k - 1 && best != 0 && (tid & 1) == 0) s_thin.tau = best;
+      __syncthreads();
+      tau = s_thin.tau;
+    }
+    bool full = false;
+    if (beam_order(mx) >= unsigned(tau >> 32)) {
+#pragma unroll
+      for (int j = 0; j < kBeamPerThread; ++j) {
+        const unsigned long long key = key_of(j);
+        if (key >= tau && key != 0) {
+          const int i = atomicAdd(&s_n, 1);
+          beam_cand[i] = key;
+          full = full || i >= kBeamKeep;
+          sum += double(expf(v[j] - base)) - double(fast_exp2((v[j] - base) * kLog2E));
+        }
+      }
+    }
+    // (the answer has to be the block's: s_n may have moved on for some)
+    full = __syncthreads_or(full);
+    if (full || w + kBeamTile >= w1) {
+      const int kept = beam_thin(beam_cand, beam_cand + kBeamRoom, s_thin, s_n, p.k);
+      if (kept == p.k) tau = beam_cand[kept - 1] + 1;  // only better ones from now on
+      if (tid == 0) s_n = kept;
+      __syncthreads();
+    }
+    raw = next;
   }
-  // the sum: expf is within 2 units in the last place; sums beyond a thread's
-  // 32 terms are held in 64 bits, since the order of two beams' candidates
-  // hangs on the last digits
-  float part = 0.f;
-  const float base = m == -INFINITY ? 0.f : m;
+  const size_t at = size_t(blockIdx.x) * p.k;
+  const int kept = w0 < w1 ? min(s_n, p.k) : 0;
+  for (int i = tid; i < p.k; i += kBeamThreads) p.keys[at + i] = i < kept ? beam_cand[i] : 0ull;
+  // the segment's maximum and sum
+  float bm = m;
 #pragma unroll
-  for (int j = 0; j < kBeamPerThread; ++j) part += expf(v[j] - base);
-  double sum = part;
+  for (int d = 1; d < 32; d <<= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, d));
+  if (lane == 0) s_max[warp] = bm;
+  __syncthreads();
+  bm = s_max[0];
+#pragma unroll
+  for (int w = 1; w < kBeamThreads / 32; ++w) bm = fmaxf(bm, s_max[w]);
+  sum = m == -INFINITY ? 0.0 : sum * double(expf(m - bm));
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   if (lane == 0) s_sum[warp] = sum;
   __syncthreads();
-  const unsigned long long tau = s_tau;
-  if (best >= tau && best != 0) {
-#pragma unroll
-    for (int j = 0; j < kBeamPerThread; ++j) {
-      const int i = j * kBeamThreads + tid;
-      if (i < count) {
-        const unsigned long long key = beam_key(v[j], i);
-        if (key >= tau) s_cand[atomicAdd(&s_n, 1)] = key;
-      }
-    }
-  }
-  __syncthreads();
-  const int n = s_n;
-  const size_t at = size_t(blockIdx.x) * p.k;
-  for (int i = tid; i < n; i += kBeamThreads) {
-    const unsigned long long mine = s_cand[i];
-    int above = 0;
-    for (int j = 0; j < n; ++j) above += s_cand[j] > mine;
-    // (the index within the chunk becomes the token)
-    if (above < p.k) p.keys[at + above] = mine - unsigned(first);
-  }
-  for (int i = n + tid; i < p.k; i += kBeamThreads) p.keys[at + i] = 0;
   if (tid == 0) {
-    double s = 0.0;
-    for (int w = 0; w < kBeamThreads / 32; ++w) s += s_sum[w];
-    p.chunk_max[blockIdx.x] = m;
-    p.chunk_sum[blockIdx.x] = s;
+    double total = 0.0;
+    for (int w = 0; w < kBeamThreads / 32; ++w) total += s_sum[w];
+    p.seg_max[blockIdx.x] = bm;
+    p.seg_sum[blockIdx.x] = total;
   }
 }
 
-// One block per request: the rows' log sums, then the k best of all chunks'
+// One block per request: the rows' log sums, then the k best of all segments'
 // lists. Lists are sorted, so the k best lie in the k lists with the best
 // heads: at most k*k candidates.
-__global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamSelectParams p) {
+__global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const BeamSelectParams p) {
   extern __shared__ unsigned long long beam_smem[];
   __shared__ double s_off[kBeamMax];
   __shared__ float s_top[kBeamMax];
@@ -172,7 +294,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamSele
   __shared__ unsigned long long s_tau_v;
   __shared__ unsigned s_tau_i;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int lists = p.beams * p.chunks;
+  const int lists = p.beams * p.segments;
   unsigned long long* head_v = beam_smem;                   // [lists] order of the head's score
   unsigned* head_i = reinterpret_cast<unsigned*>(head_v + lists);  // [lists] its beam*vocab + token
   unsigned long long* cand_v = head_v + lists + (lists + 1) / 2;
@@ -180,16 +302,16 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamSele
   grid_launch_dependents();
   grid_dependency_wait();
   const int b = blockIdx.x;
-  for (int w = warp; w < p.beams; w += kBeamThreads / 32) {
-    const size_t at = (size_t(b) * p.beams + w) * p.chunks;
+  for (int w = warp; w < p.beams; w += kBeamMergeThreads / 32) {
+    const size_t at = (size_t(b) * p.beams + w) * p.segments;
     float m = -INFINITY;
-    for (int c = lane; c < p.chunks; c += 32) m = fmaxf(m, p.chunk_max[at + c]);
+    for (int c = lane; c < p.segments; c += 32) m = fmaxf(m, p.seg_max[at + c]);
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     double s = 0.0;
     if (m != -INFINITY)
-      for (int c = lane; c < p.chunks; c += 32)
-        s += p.chunk_sum[at + c] * exp(double(p.chunk_max[at + c]) - double(m));
+      for (int c = lane; c < p.segments; c += 32)
+        s += p.seg_sum[at + c] * exp(double(p.seg_max[at + c]) - double(m));
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
     // a row without a possible token, and a beam that is out, give -inf
@@ -209,22 +331,22 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamSele
   // A candidate's score (logit - largest first: a row of lowest values, as
   // masks leave it, would swallow the rest)
   auto value = [&](int list, unsigned long long key) -> unsigned long long {
-    const int w = list / p.chunks;
+    const int w = list / p.segments;
     return beam_order64(s_off[w] + (double(beam_value(unsigned(key >> 32))) - double(s_top[w])));
   };
   auto index = [&](int list, unsigned long long key) -> unsigned {
-    return unsigned(list / p.chunks) * unsigned(p.vocab) + (0xffffffffu - unsigned(key));
+    return unsigned(list / p.segments) * unsigned(p.vocab) + (0xffffffffu - unsigned(key));
   };
   auto before = [](unsigned long long va, unsigned ia, unsigned long long vb, unsigned ib) {
     return va > vb || (va == vb && ia < ib);
   };
-  for (int l = tid; l < lists; l += kBeamThreads) {
+  for (int l = tid; l < lists; l += kBeamMergeThreads) {
     const unsigned long long key = keys[size_t(l) * p.k];
     head_v[l] = value(l, key);
     head_i[l] = index(l, key);
   }
   __syncthreads();
-  for (int l = tid; l < lists; l += kBeamThreads) {  // the k-th best head
+  for (int l = tid; l < lists; l += kBeamMergeThreads) {  // the k-th best head
     const unsigned long long v = head_v[l];
     const unsigned id = head_i[l];
     int above = 0;
@@ -237,7 +359,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamSele
   __syncthreads();
   const unsigned long long tau_v = s_tau_v;
   const unsigned tau_i = s_tau_i;
-  for (int e = tid; e < lists * p.k; e += kBeamThreads) {
+  for (int e = tid; e < lists * p.k; e += kBeamMergeThreads) {
     const int l = e / p.k;
     if (before(tau_v, tau_i, head_v[l], head_i[l])) continue;  // a list behind the k best heads
     const unsigned long long key = keys[e];
@@ -251,7 +373,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamSele
   }
   __syncthreads();
   const int n = s_n;
-  for (int i = tid; i < n; i += kBeamThreads) {
+  for (int i = tid; i < n; i += kBeamMergeThreads) {
     const unsigned long long v = cand_v[i];
     const unsigned id = cand_i[i];
     int above = 0;
@@ -281,49 +403,60 @@ struct BeamReorderParams {
   int* pages_out;            // [batch, beams_out, max_pages], not pages_in
   int* lengths_out;          // [batch, beams_out], not lengths_in
   unsigned* marks;           // workspace [batch * beams_in, words]
-  int* children;             // workspace [batch * beams_in]
   unsigned* err;
 };
 
-constexpr int kReorderThreads = 256;
+constexpr int kReorderWarps = 4;
 constexpr int kReleaseThreads = 1024;
+constexpr int kReleaseList = 256;  // freed pages of a warp that fit in shared memory
+constexpr size_t kReleaseSmem = size_t(kReleaseThreads / 32) * kReleaseList * sizeof(int2);
 
-// Blocks [0, row_blocks): a warp per (request, 32 columns) writes the new rows
-// and marks, in each column, the last beam that holds a page whose reference
-// count changes. The other blocks copy the state where it is not updated in
-// place.
-__global__ void __launch_bounds__(kReorderThreads)
-    beam_rows_kernel(const BeamReorderParams p, int row_blocks) {
-  __shared__ int s_child[kReorderThreads / 32][kBeamMax];
-  __shared__ int s_parent[kReorderThreads / 32][kBeamMax];
-  __shared__ int s_pages[kReorderThreads / 32][kBeamMax];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// The state's copies, where it is not updated in place.
+__global__ void __launch_bounds__(256) pool_copy_kernel(int n, const int* __restrict__ a, int* a_out,
+                                                        const int* __restrict__ b, int* b_out) {
   grid_launch_dependents();
   grid_dependency_wait();
-  if (int(blockIdx.x) >= row_blocks) {
-    const int at = (int(blockIdx.x) - row_blocks) * kReorderThreads + tid;
-    const int step = (int(gridDim.x) - row_blocks) * kReorderThreads;
-    if (p.refcount != p.refcount_in)
-      for (int i = at; i < p.physical_pages; i += step) p.refcount[i] = p.refcount_in[i];
-    if (p.free_stack != p.free_stack_in)
-      for (int i = at; i < p.physical_pages; i += step) p.free_stack[i] = p.free_stack_in[i];
-    return;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) {
+    if (a_out != a) a_out[i] = a[i];
+    if (b_out != b) b_out[i] = b[i];
   }
-  const long long item = (long long)blockIdx.x * (kReorderThreads / 32) + warp;
+}
+
+// A warp per (request, 32 columns): the old entries are read once, the new rows
+// written; a page's reference count changes by its holders' children less one
+// each, once per column, and where that is a loss the last beam holding it is
+// marked (the page may be free now). Most columns are one page held by all beams,
+// as many before as after: nothing to do.
+__global__ void __launch_bounds__(kReorderWarps * 32) beam_rows_kernel(const BeamReorderParams p) {
+  __shared__ int s_child[kReorderWarps][kBeamMax];
+  __shared__ int s_parent[kReorderWarps][kBeamMax];
+  __shared__ int s_pages[kReorderWarps][kBeamMax][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const long long item = (long long)blockIdx.x * kReorderWarps + warp;
   if (item >= (long long)p.batch * p.words) return;
   const int b = int(item / p.words), word = int(item % p.words), c = word * 32 + lane;
   int* child = s_child[warp];
   int* parent = s_parent[warp];
-  int* held = s_pages[warp];  // page counts of the rows
-  for (int r = lane; r < p.beams_in; r += 32) {
-    int len = p.lengths_in[size_t(b) * p.beams_in + r];
-    if (len < 0 || len > p.max_pages * kPageSize) {
-      atomicOr(p.err, kErrLength);
-      len = len < 0 ? 0 : p.max_pages * kPageSize;
+  int (*page)[32] = s_pages[warp];
+  const bool col = c < p.max_pages;
+  const int* in = p.pages_in + size_t(b) * p.beams_in * p.max_pages + c;
+  bool bad_page = false;
+#pragma unroll 8
+  for (int r = 0; r < p.beams_in; ++r) {
+    const int raw = p.lengths_in[size_t(b) * p.beams_in + r];
+    const int len = min(max(raw, 0), p.max_pages * kPageSize);
+    if (raw != len && lane == 0) atomicOr(p.err, kErrLength);
+    int id = -1;
+    if (col && c < (len + kPageSize - 1) / kPageSize) {
+      id = in[size_t(r) * p.max_pages];
+      bad_page |= id < 0 || id >= p.physical_pages;
     }
-    held[r] = (len + kPageSize - 1) / kPageSize;
-    child[r] = 0;
+    page[r][lane] = id;
   }
+  if (bad_page) atomicOr(p.err, kErrPageRange);
+  for (int r = lane; r < p.beams_in; r += 32) child[r] = 0;
   __syncwarp();
   for (int j = lane; j < p.beams_out; j += 32) {
     int r = p.parents[size_t(b) * p.beams_out + j];
@@ -337,115 +470,139 @@ __global__ void __launch_bounds__(kReorderThreads)
       p.lengths_out[size_t(b) * p.beams_out + j] = r < 0 ? 0 : p.lengths_in[size_t(b) * p.beams_in + r];
   }
   __syncwarp();
-  if (word == 0)
-    for (int r = lane; r < p.beams_in; r += 32) p.children[size_t(b) * p.beams_in + r] = child[r];
-  const int* in = p.pages_in + size_t(b) * p.beams_in * p.max_pages + c;
-  const bool col = c < p.max_pages;
-  auto page_of = [&](int r) -> int {
-    return col && c < held[r] ? in[size_t(r) * p.max_pages] : -1;
-  };
-  for (int j = 0; j < p.beams_out; ++j)
-    if (col)
-      p.pages_out[(size_t(b) * p.beams_out + j) * p.max_pages + c] = parent[j] < 0 ? -1 : page_of(parent[j]);
+  if (col)
+    for (int j = 0; j < p.beams_out; ++j)
+      p.pages_out[(size_t(b) * p.beams_out + j) * p.max_pages + c] =
+          parent[j] < 0 ? -1 : page[parent[j]][lane];
+  // (children of all rows less rows: the change of a page that all hold)
+  int all = -p.beams_in;
+  for (int r = 0; r < p.beams_in; ++r) all += child[r];
+  bool same = true;
+  for (int r = 1; r < p.beams_in; ++r) same = same && page[r][lane] == page[0][lane];
+  const bool quiet = same && (all == 0 || page[0][lane] < 0);
+  const bool none = __all_sync(0xffffffffu, quiet);
   for (int r = 0; r < p.beams_in; ++r) {
-    const int page = page_of(r);
     bool mark = false;
-    if (page >= 0 && page < p.physical_pages) {
+    const int id = page[r][lane];
+    if (!quiet && id >= 0 && id < p.physical_pages) {
       int net = child[r] - 1;
-      mark = true;
+      bool last = true;
       for (int o = 0; o < p.beams_in; ++o)
-        if (o != r && page_of(o) == page) {
+        if (o != r && page[o][lane] == id) {
           net += child[o] - 1;
-          if (o > r) mark = false;  // a later beam holds it too
+          last = last && o < r;
         }
-      mark = mark && net != 0;
-    } else if (col && c < held[r]) {
-      atomicOr(p.err, kErrPageRange);
+      if (last && net != 0) atomicAdd(&p.refcount[id], net);
+      mark = last && net < 0;
     }
-    const unsigned bits = __ballot_sync(0xffffffffu, mark);
+    const unsigned bits = none ? 0u : __ballot_sync(0xffffffffu, mark);
     if (lane == 0) p.marks[(size_t(b) * p.beams_in + r) * p.words + word] = bits;
   }
 }
 
-// One block: applies the marked changes, then pushes the pages nobody holds
-// any more in the order of their last release (row, then column). A page that
-// beams of two requests held (a common prompt) may be marked in both: the
-// later mark claims it, by writing its place into the zero reference count.
+// One block: of the marked pages, those that nobody holds any more are pushed in
+// the order of their last release (row, then column). A page that beams of two
+// requests held (a common prompt) may be marked in both: the later mark claims it,
+// by writing its place into the zero reference count. Every warp takes a run of
+// words of the marks, its freed pages listed in order in shared memory; where a
+// list runs over, all warps go through the marks themselves instead.
 __global__ void __launch_bounds__(kReleaseThreads) beam_release_kernel(const BeamReorderParams p) {
+  extern __shared__ int2 release_list[];
   __shared__ int s_warp[kReleaseThreads / 32];
+  __shared__ int s_over;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int kWarps = kReleaseThreads / 32;
   grid_launch_dependents();
+  if (tid == 0) s_over = 0;
   grid_dependency_wait();
+  __syncthreads();
   const long long total = (long long)p.batch * p.beams_in * p.words;
-  const long long per = (total + kReleaseThreads - 1) / kReleaseThreads;
-  const long long w0 = min(total, tid * per), w1 = min(total, w0 + per);
+  const long long per = (total + kWarps - 1) / kWarps;
+  const long long w0 = min(total, warp * per), w1 = min(total, w0 + per);
   auto page_at = [&](long long w, int bit) -> int {
     return p.pages_in[size_t(w / p.words) * p.max_pages + size_t(w % p.words) * 32 + bit];
   };
-  for (long long w = w0; w < w1; ++w) {
-    for (unsigned bits = p.marks[w]; bits; bits &= bits - 1) {
-      const int bit = __ffs(bits) - 1, page = page_at(w, bit);
-      const long long row = w / p.words;
-      const int b = int(row / p.beams_in), c = int(w % p.words) * 32 + bit;
-      int net = 0;
-      for (int r = 0; r < p.beams_in; ++r) {
-        const size_t at = size_t(b) * p.beams_in + r;
-        const int len = min(max(p.lengths_in[at], 0), p.max_pages * kPageSize);
-        if (c < (len + kPageSize - 1) / kPageSize && p.pages_in[at * p.max_pages + c] == page)
-          net += p.children[at] - 1;
+  auto count_of = [&](int page) { return *reinterpret_cast<volatile int*>(&p.refcount[page]); };
+  const int count = *p.free_count_in;
+
+  // the marked pages that became free: their marks stay, and they are listed
+  int2* list = release_list + warp * kReleaseList;  // (place, page)
+  int n = 0;
+  for (long long g = w0; g < w1; g += 32) {
+    const unsigned word = g + lane < w1 ? p.marks[g + lane] : 0u;
+    unsigned some = __ballot_sync(0xffffffffu, word != 0u);
+    while (some) {  // four words of marks at a time, a lane a bit
+      int src[4], page[4], rc[4];
+      unsigned bits[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        src[i] = some ? __ffs(some) - 1 : -1;
+        bits[i] = __shfl_sync(0xffffffffu, word, max(src[i], 0));
+        if (src[i] < 0) bits[i] = 0u;
+        some &= some - 1;
+        page[i] = (bits[i] >> lane) & 1u ? page_at(g + src[i], lane) : -1;
       }
-      atomicAdd(&p.refcount[page], net);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rc[i] = page[i] >= 0 ? count_of(page[i]) : 1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned left = __ballot_sync(0xffffffffu, rc[i] == 0);
+        const int at = n + __popc(left & ((1u << lane) - 1));
+        if (rc[i] == 0 && at < kReleaseList) list[at] = make_int2(int((g + src[i]) * 32 + lane), page[i]);
+        n += __popc(left);
+        if (lane == 0 && src[i] >= 0 && left != bits[i]) p.marks[g + src[i]] = left;
+      }
     }
   }
+  if (n > kReleaseList && lane == 0) s_over = 1;
   __syncthreads();
-  for (long long w = w0; w < w1; ++w) {  // keep the marks of pages that became free
-    unsigned left = 0;
-    const unsigned was = p.marks[w];
-    for (unsigned bits = was; bits; bits &= bits - 1) {
-      const int bit = __ffs(bits) - 1;
-      if (*reinterpret_cast<volatile int*>(&p.refcount[page_at(w, bit)]) == 0) left |= 1u << bit;
+  const bool listed = s_over == 0;
+  // what is left, in order: (place, page) of this lane's next entry, or none
+  auto each = [&](auto&& f) {
+    if (listed) {
+      for (int i0 = 0; i0 < n; i0 += 32) {
+        const bool in = i0 + lane < n;
+        const int2 e = in ? list[i0 + lane] : make_int2(0, 0);
+        f(in, e.x, e.y);
+      }
+    } else {
+      for (long long w = w0; w < w1; ++w) {
+        const unsigned bits = p.marks[w];
+        if (bits == 0u) continue;
+        const bool in = (bits >> lane) & 1u;
+        f(in, int(w * 32 + lane), in ? page_at(w, lane) : 0);
+      }
     }
-    if (left != was) p.marks[w] = left;
-  }
-  __syncthreads();
-  for (long long w = w0; w < w1; ++w)
-    for (unsigned bits = p.marks[w]; bits; bits &= bits - 1) {
-      const int bit = __ffs(bits) - 1;
-      atomicMin(&p.refcount[page_at(w, bit)], -int(w * 32 + bit) - 1);
-    }
+  };
+  each([&](bool in, int place, int page) {
+    if (in) atomicMin(&p.refcount[page], -place - 1);
+  });
   __syncthreads();
   int mine = 0;
-  for (long long w = w0; w < w1; ++w)
-    for (unsigned bits = p.marks[w]; bits; bits &= bits - 1) {
-      const int bit = __ffs(bits) - 1;
-      mine += *reinterpret_cast<volatile int*>(&p.refcount[page_at(w, bit)]) == -int(w * 32 + bit) - 1;
-    }
-  int scan = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, scan, d);
-    if (lane >= d) scan += up;
-  }
-  if (lane == 31) s_warp[warp] = scan;
-  const int count = *p.free_count_in;
+  each([&](bool in, int place, int page) {
+    mine += __popc(__ballot_sync(0xffffffffu, in && count_of(page) == -place - 1));
+  });
+  if (lane == 0) s_warp[warp] = mine;
   __syncthreads();
-  int before = scan - mine, freed = 0;
-  for (int w = 0; w < kReleaseThreads / 32; ++w) {
+  int before = 0, freed = 0;
+  for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += s_warp[w];
     freed += s_warp[w];
   }
-  for (long long w = w0; w < w1; ++w)
-    for (unsigned bits = p.marks[w]; bits; bits &= bits - 1) {
-      const int bit = __ffs(bits) - 1, page = page_at(w, bit);
-      if (*reinterpret_cast<volatile int*>(&p.refcount[page]) != -int(w * 32 + bit) - 1) continue;
-      const long long at = (long long)count + before++;
+  each([&](bool in, int place, int page) {
+    const bool won = in && count_of(page) == -place - 1;
+    const unsigned wins = __ballot_sync(0xffffffffu, won);
+    if (won) {
+      const long long at = (long long)count + before + __popc(wins & ((1u << lane) - 1));
       if (at >= 0 && at < p.physical_pages)
         p.free_stack[at] = page;
       else
         atomicOr(p.err, kErrPageRange);
       p.refcount[page] = 0;
     }
-  if (tid == 0) *p.free_count = min(count + freed, p.physical_pages);
+    before += __popc(wins);
+  });
+  if (tid == 0) *p.free_count = int(min((long long)count + freed, (long long)p.physical_pages));
 }
 
 }  // namespace bc

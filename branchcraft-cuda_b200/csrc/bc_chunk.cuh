@@ -41,6 +41,7 @@
 namespace bc {
 
 constexpr int kChThreads = 384;
+constexpr int kChMergeThreads = 256;
 constexpr int kChTile = 128;      // keys of a tile: eight pages
 constexpr int kChDescs = 4;       // item descriptors in flight
 constexpr int kChMaxBatch = 4096;
@@ -248,21 +249,6 @@ __device__ __forceinline__ void add_pair(float& a0, float& a1, float b0, float b
       : "f"(b0), "f"(b1));
 }
 
-__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 // Largest magnitude of three.
 __device__ __forceinline__ float fmax3_abs(float a, float b, float c) {
   float r;
@@ -417,8 +403,9 @@ __global__ void __launch_bounds__(kChThreads, 1)
       // ---------------------------------------------------------- scheduler
       // This block's share: from its own cut (found by lanes 0-15) up to the next
       // block's (lanes 16-31). Cuts inside an item fall on multiples of `grain`
-      // tiles from its start (a thirty-second of a share, at least kChMinPiece: a
-      // piece costs its partial state's way through memory) or on its ends.
+      // tiles from its start (a thirty-second of a share; at least kChMinPiece, half
+      // that in large shares: a piece costs its partial state's way through memory)
+      // or on its ends.
       const int half = lane >> 4, hl = lane & 15;
       const int per_lane = (p.batch + 15) / 16;
       const int sb0 = min(p.batch, hl * per_lane), sb1 = min(p.batch, sb0 + per_lane);
@@ -469,12 +456,15 @@ __global__ void __launch_bounds__(kChThreads, 1)
       rem -= __shfl_sync(0xffffffffu, at, src, 16) * p.hkv;
       // its head and tile
       const int weight = chunk_weight(p, r.n - blk * block_tokens);
-      const int grain = max(kChMinPiece, int(min(cost / gridDim.x / (32 * weight), 1ll << 20)));
+      const long long share = cost / (gridDim.x * weight);  // in this item's tiles
+      const int grain = max(share >= 4 * kChMinPiece ? kChMinPiece / 2 : kChMinPiece,
+                            int(min(share / 32, 1ll << 20)));
       if (in) {
         head = int(double(rem) / double(n));
         off = max(int(rem - (long long)head * n) - kChItemCost, 0) / weight;
         n = (n - kChItemCost) / weight;
-        off = (off + grain / 2) / grain * grain;
+        // (an item of no more than a piece and a tile stays whole)
+        off = n <= kChMinPiece + 1 ? (2 * off > n ? n : 0) : (off + grain / 2) / grain * grain;
         if (off > 0 && n - off < (grain + 1) / 2) {  // the next item's start
           off = 0;
           if (++head == p.hkv) {
@@ -1107,7 +1097,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
 // blockIdx.x: its own, then those of the following blocks up to the one that
 // ends it, 32 rows per block of blockIdx.y.
 template <int D, typename T>
-__global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkParams p) {
+__global__ void __launch_bounds__(kChMergeThreads) chunk_merge_kernel(const ChunkParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   grid_launch_dependents();
   grid_dependency_wait();
@@ -1122,7 +1112,7 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkParams p) {
   // Where the pieces lie, 32 blocks looked at together: those after c that have a
   // share, up to the one that ends the item.
   constexpr int kMost = 160;  // (a block per SM)
-  __shared__ int s_slot[4][kMost];
+  __shared__ int s_slot[kChMergeThreads / 32][kMost];
   int* slot = s_slot[warp];
   int n = 1;
   if (lane == 0) slot[0] = c * 2 + 1;
@@ -1138,25 +1128,51 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkParams p) {
   }
   __syncwarp();
   if (!valid) return;
+  // Online over the pieces, in order, four pieces' loads in flight together.
+  constexpr int N = D / 32;  // float4 pieces of a warp
+  constexpr int F = 4;
   float m = -INFINITY, l = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) m = fmaxf(m, p.part_ml[size_t(slot[i]) * p.part_rows + row].x);
-  constexpr int N = D / 16;  // float4 pieces of a warp
   float4 acc[N];
 #pragma unroll
   for (int q = 0; q < N; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-  for (int i = 0; i < n; ++i) {
-    const float2 ml = p.part_ml[size_t(slot[i]) * p.part_rows + row];
-    const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - m);  // (O of such a piece is 0)
-    l += w * ml.y;
+  for (int i0 = 0; i0 < n; i0 += F) {
+    float2 ml[F];
+    float4 o[F][N];
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      const bool in = i0 + i < n;
+      const size_t at = in ? size_t(slot[i0 + i]) : 0;
+      ml[i] = in ? p.part_ml[at * p.part_rows + row] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int q = 0; q < N; ++q)
+        o[i][q] = in ? p.part_o[(at * (D / 4) + warp * N + q) * p.part_rows + row]
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < F; ++i) mn = fmaxf(mn, ml[i].x);
+    const float a = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+    m = mn;
+    l *= a;
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      const float4 o = p.part_o[(size_t(slot[i]) * (D / 4) + warp * N + q) * p.part_rows + row];
-      acc[q].x += w * o.x;
-      acc[q].y += w * o.y;
-      acc[q].z += w * o.z;
-      acc[q].w += w * o.w;
+      acc[q].x *= a;
+      acc[q].y *= a;
+      acc[q].z *= a;
+      acc[q].w *= a;
+    }
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      // (a piece without keys has O = 0)
+      const float w = ml[i].x == -INFINITY ? 0.f : fast_exp2(ml[i].x - m);
+      l += w * ml[i].y;
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        acc[q].x += w * o[i][q].x;
+        acc[q].y += w * o[i][q].y;
+        acc[q].z += w * o[i][q].z;
+        acc[q].w += w * o[i][q].w;
+      }
     }
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;

@@ -1131,8 +1131,7 @@ struct ChunkPlan {
     const long long items = ((long long)tokens / (2 * tile) + std::min(s->batch, tokens)) * s->kv_heads;
     blocks = int(std::min<long long>(std::min(dev < 0 ? 148 : sm_count(dev), 160), items * key_tiles));
     rows = tokens <= tile ? (tokens * group + 31) / 32 * 32 : 256;
-    // (cuts fall on multiples of kChMinPiece tiles and leave at least half of
-    // that: an item of kChMinPiece + 1 tiles is never split)
+    // (an item of kChMinPiece + 1 tiles is never split)
     bytes = key_tiles <= kChMinPiece + 1
                 ? 0
                 : size_t(blocks) * (2 * size_t(rows) * (s->dim * 4 + 8) + 32);
@@ -1161,7 +1160,8 @@ cudaError_t launch_chunk_mod(ChunkParams& p, const CUtensorMap* maps, const Chun
                                    maps[0], maps[1], maps[2]);
   if (e != cudaSuccess || plan.bytes == 0) return e;
   return launch_dependent(chunk_merge_kernel<D, T>,
-                          dim3(unsigned(plan.blocks), unsigned((plan.rows + 31) / 32)), 128, 0,
+                          dim3(unsigned(plan.blocks), unsigned((plan.rows + 31) / 32)),
+                          kChMergeThreads, 0,
                           stream, p);
 }
 
@@ -1176,14 +1176,37 @@ cudaError_t launch_chunk(ChunkParams& p, const CUtensorMap* maps, const ChunkPla
   }
 }
 
+// Rows are cut into the number of segments that takes the least time by count:
+// waves of four blocks a SM times a segment's steps and its fixed work (the first
+// bound and the last ranking, some four steps' time).
+struct BeamPlan {
+  int segments, segment;
+  BeamPlan(int rows, int vocab, int dev) {
+    const int steps = (vocab + 15 + kBeamTile - 1) / kBeamTile;  // (from a 16-byte boundary on)
+    const long long slots = 4ll * (dev < 0 ? 148 : sm_count(dev));
+    long long least = -1;
+    int per = steps;
+    for (int s = 1; s <= steps && (s == 1 || (long long)rows * s <= 4 * slots); ++s) {
+      const int each = (steps + s - 1) / s;
+      const long long time = (((long long)rows * s + slots - 1) / slots) * (each + 4);
+      if (least < 0 || time < least) {
+        least = time;
+        per = each;
+      }
+    }
+    segment = per * kBeamTile;
+    segments = (vocab + 15 + segment - 1) / segment;
+  }
+};
+
 template <typename T>
-cudaError_t launch_beam_chunks(const BeamSelectParams& p, int dev, cudaStream_t stream) {
+cudaError_t launch_beam_segments(const BeamSelectParams& p, int dev, cudaStream_t stream) {
   static std::atomic<uint64_t> configured{0};
-  const auto smem = [](int k) { return size_t(k) * 4 * kBeamPerThread * 8; };
-  const cudaError_t e = raise_smem(beam_chunk_kernel<T>, smem(kBeamMaxK), configured, dev);
+  constexpr size_t smem = size_t(kBeamRoom + kBeamThinned) * 8;
+  const cudaError_t e = raise_smem(beam_segment_kernel<T>, smem, configured, dev);
   if (e != cudaSuccess) return e;
-  return launch_dependent(beam_chunk_kernel<T>, dim3(unsigned(p.batch) * p.beams * p.chunks),
-                          kBeamThreads, smem(p.k), stream, p);
+  return launch_dependent(beam_segment_kernel<T>, dim3(unsigned(p.batch) * p.beams * p.segments),
+                          kBeamThreads, smem, stream, p);
 }
 
 size_t beam_merge_smem(long long lists, int k) {
@@ -1193,10 +1216,8 @@ size_t beam_merge_smem(long long lists, int k) {
 bool beam_shape_ok(int batch, int beams, int vocab, int k) {
   return batch >= 1 && beams >= 1 && beams <= kBeamMax && vocab >= 1 && vocab <= kBeamMaxVocab &&
          k >= 1 && k <= kBeamMaxK && k <= (long long)beams * vocab &&
-         (long long)batch * beams * ((vocab + kBeamChunk - 1) / kBeamChunk) <= 0x7fffffff;
+         (long long)batch * beams <= 0xffffff;
 }
-
-int beam_chunks(int vocab) { return (vocab + kBeamChunk - 1) / kBeamChunk; }
 
 bool reorder_shape_ok(int batch, int beams_in, int max_pages) {
   return batch >= 1 && beams_in >= 1 && beams_in <= kBeamMax && max_pages >= 1 &&
@@ -1359,8 +1380,9 @@ int bc_chunk_attention(const bc_shape* s, int tokens, int dtype, const void* q,
 
 size_t bc_beam_workspace_bytes(int batch, int beams, int vocab, int k) {
   if (!beam_shape_ok(batch, beams, vocab, k)) return 0;
-  // per chunk: k keys, its sum and its largest logit
-  return size_t(batch) * beams * beam_chunks(vocab) * (size_t(k) * 8 + 8 + 4);
+  // per segment: k keys, its sum and its largest logit
+  const BeamPlan plan(batch * beams, vocab, current_device());
+  return size_t(batch) * beams * plan.segments * (size_t(k) * 8 + 8 + 4);
 }
 
 int bc_beam_select(int batch, int beams, int vocab, int k, int dtype, const void* logits,
@@ -1380,34 +1402,36 @@ int bc_beam_select(int batch, int beams, int vocab, int k, int dtype, const void
   p.beams = beams;
   p.vocab = vocab;
   p.k = k;
-  p.chunks = beam_chunks(vocab);
+  const BeamPlan plan(batch * beams, vocab, dev);
+  p.segments = plan.segments;
+  p.segment = plan.segment;
   p.logits = logits;
   p.row_stride = row_stride;
   p.scores = scores;
   p.out_scores = out_scores;
   p.out_tokens = out_tokens;
   p.out_parents = out_parents;
-  const size_t lists = size_t(batch) * beams * p.chunks;
+  const size_t lists = size_t(batch) * beams * p.segments;
   p.keys = static_cast<unsigned long long*>(workspace);
-  p.chunk_sum = reinterpret_cast<double*>(p.keys + lists * k);
-  p.chunk_max = reinterpret_cast<float*>(p.chunk_sum + lists);
+  p.seg_sum = reinterpret_cast<double*>(p.keys + lists * k);
+  p.seg_max = reinterpret_cast<float*>(p.seg_sum + lists);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = dtype == BC_F16    ? launch_beam_chunks<__half>(p, dev, st)
-                  : dtype == BC_BF16 ? launch_beam_chunks<__nv_bfloat16>(p, dev, st)
-                                     : launch_beam_chunks<float>(p, dev, st);
+  cudaError_t e = dtype == BC_F16    ? launch_beam_segments<__half>(p, dev, st)
+                  : dtype == BC_BF16 ? launch_beam_segments<__nv_bfloat16>(p, dev, st)
+                                     : launch_beam_segments<float>(p, dev, st);
   if (e != cudaSuccess) return e;
   static std::atomic<uint64_t> configured{0};
-  e = raise_smem(beam_merge_kernel,
-                 beam_merge_smem((long long)kBeamMax * beam_chunks(kBeamMaxVocab), kBeamMaxK),
+  // (a request's lists: at most sixteen blocks a SM, or one a beam)
+  e = raise_smem(beam_merge_kernel, beam_merge_smem(std::max(16 * sm_count(dev), kBeamMax), kBeamMaxK),
                  configured, dev);
   if (e != cudaSuccess) return e;
-  return launch_dependent(beam_merge_kernel, dim3(unsigned(batch)), kBeamThreads,
-                          beam_merge_smem((long long)beams * p.chunks, k), st, p);
+  return launch_dependent(beam_merge_kernel, dim3(unsigned(batch)), kBeamMergeThreads,
+                          beam_merge_smem((long long)beams * p.segments, k), st, p);
 }
 
 size_t bc_reorder_workspace_bytes(int batch, int beams_in, int max_pages) {
   if (!reorder_shape_ok(batch, beams_in, max_pages)) return 0;
-  return size_t(batch) * beams_in * ((max_pages + 31) / 32 + 1) * 4;
+  return size_t(batch) * beams_in * ((max_pages + 31) / 32) * 4;
 }
 
 int bc_beam_reorder(int batch, int beams_in, int beams_out, int physical_pages,
@@ -1446,18 +1470,18 @@ int bc_beam_reorder(int batch, int beams_in, int beams_out, int physical_pages,
   p.pages_out = pages_out;
   p.lengths_out = lengths_out;
   p.marks = static_cast<unsigned*>(workspace);
-  p.children = static_cast<int*>(workspace) + size_t(batch) * beams_in * p.words;
   p.err = err;
-  const int warps = kReorderThreads / 32;
-  const int row_blocks = int(((long long)batch * p.words + warps - 1) / warps);
-  const bool copy = refcount != refcount_in || free_stack != free_stack_in;
-  const int copiers =
-      copy ? std::min(64, (physical_pages + 4 * kReorderThreads - 1) / (4 * kReorderThreads)) : 0;
+  const int row_blocks = int(((long long)batch * p.words + kReorderWarps - 1) / kReorderWarps);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = launch_dependent(beam_rows_kernel, dim3(unsigned(row_blocks + copiers)),
-                                         kReorderThreads, 0, st, p, row_blocks);
+  static std::atomic<uint64_t> configured{0};
+  cudaError_t e = raise_smem(beam_release_kernel, kReleaseSmem, configured, dev);
+  if (e == cudaSuccess && (refcount != refcount_in || free_stack != free_stack_in))
+    e = launch_dependent(pool_copy_kernel, dim3(unsigned(std::min(256, (physical_pages + 255) / 256))),
+                         256, 0, st, physical_pages, refcount_in, refcount, free_stack_in, free_stack);
+  if (e == cudaSuccess)
+    e = launch_dependent(beam_rows_kernel, dim3(unsigned(row_blocks)), kReorderWarps * 32, 0, st, p);
   if (e != cudaSuccess) return e;
-  return launch_dependent(beam_release_kernel, dim3(1), kReleaseThreads, 0, st, p);
+  return launch_dependent(beam_release_kernel, dim3(1), kReleaseThreads, kReleaseSmem, st, p);
 }
 
 int bc_selftest_bounded_wait(int ctas, int smem_bytes, unsigned limit_us, void* stream) {

@@ -14,6 +14,7 @@
 // Every op calls the C ABI (branchcraft.h) on the current CUDA stream.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -290,6 +291,11 @@ void commit_batch_cuda(at::Tensor& cache_k, at::Tensor& cache_v, const at::Tenso
 
 using at::Tensor;
 
+// (past the dispatcher: a step's small outputs cost the host more than the GPU)
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 void check_state(const Tensor& pages, const Tensor& lengths, const Tensor& refcount,
                  const Tensor& free_stack, const Tensor& free_count) {
   for (const auto& [t, name] : {std::pair<const Tensor&, const char*>{pages, "pages"},
@@ -313,13 +319,12 @@ PlanOutputs run_append_plan(const Tensor& pages, const Tensor& lengths, const Te
                             Tensor refcount_out, Tensor free_stack_out, Tensor free_count_out,
                             int64_t max_tokens, const char* op) {
   const int64_t batch = pages.size(0);
-  auto i32 = pages.options();
-  auto query_start = at::empty({batch + 1}, i32);
-  auto slot_map = at::empty({max_tokens}, i32);
-  auto positions = at::empty({max_tokens}, i32);
-  auto clones = at::empty({3, batch}, i32);
-  auto counts = at::empty({3}, i32);
-  auto scratch = at::empty({batch + 1}, i32);
+  auto query_start = fresh({batch + 1}, at::kInt, pages);
+  auto slot_map = fresh({max_tokens}, at::kInt, pages);
+  auto positions = fresh({max_tokens}, at::kInt, pages);
+  auto clones = fresh({3, batch}, at::kInt, pages);
+  auto counts = fresh({3}, at::kInt, pages);
+  auto scratch = fresh({batch + 1}, at::kInt, pages);
   check_launch(
       bc_append_plan(int(batch), int(refcount.numel()), pages.data_ptr<int>(), int(pages.size(1)),
                      lengths.data_ptr<int>(), new_tokens.data_ptr<int>(),
@@ -357,10 +362,12 @@ append_plan_cuda(const Tensor& pages, const Tensor& lengths, const Tensor& new_t
   check_append_plan(pages, lengths, new_tokens, refcount, free_stack, free_count, max_tokens,
                     max_pages);
   const c10::cuda::CUDAGuard guard(pages.device());
-  auto pages_out = at::empty({pages.size(0), max_pages > 0 ? max_pages : pages.size(1)},
-                             pages.options());
-  auto lengths_out = at::empty_like(lengths), refcount_out = at::empty_like(refcount),
-       stack_out = at::empty_like(free_stack), count_out = at::empty_like(free_count);
+  auto pages_out =
+      fresh({pages.size(0), max_pages > 0 ? max_pages : pages.size(1)}, at::kInt, pages);
+  auto lengths_out = fresh(lengths.sizes(), at::kInt, pages),
+       refcount_out = fresh(refcount.sizes(), at::kInt, pages),
+       stack_out = fresh(free_stack.sizes(), at::kInt, pages),
+       count_out = fresh(free_count.sizes(), at::kInt, pages);
   auto [qs, sm, pos, cl, cn] =
       run_append_plan(pages, lengths, new_tokens, refcount, free_stack, free_count, pages_out,
                       lengths_out, refcount_out, stack_out, count_out, max_tokens, "append_plan");
@@ -481,7 +488,7 @@ void run_chunk(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& 
   const bc_shape s{int(batch), int(hq), int(hkv), int(q.size(2)), int(pages.size(1)),
                    int(k.size(0))};
   const size_t bytes = bc_chunk_workspace_bytes(&s, int(tokens));
-  auto workspace = at::empty({int64_t(bytes)}, q.options().dtype(at::kByte));
+  auto workspace = fresh({int64_t(bytes)}, at::kByte, q);
   check_launch(bc_chunk_attention(&s, int(tokens), q.scalar_type() == at::kHalf ? BC_F16 : BC_BF16,
                                   q.data_ptr(), token_stride(q), k.data_ptr(), v.data_ptr(), &layout,
                                   pages.data_ptr<int>(), query_start.data_ptr<int>(),
@@ -497,7 +504,8 @@ Tensor chunk_attention_cuda(const Tensor& q, const Tensor& k, const Tensor& v, c
                             const std::optional<Tensor>& alibi_slopes,
                             const std::optional<Tensor>& prefix,
                             const std::optional<Tensor>& key_start) {
-  auto output = at::empty(q.sizes(), q.options());
+  TORCH_CHECK(q.is_cuda(), "q must be CUDA");
+  auto output = fresh(q.sizes(), q.scalar_type(), q);
   run_chunk(q, k, v, pages, query_start, lengths, output, scale, softcap, window, alibi_slopes,
             prefix, key_start, "chunk_attention");
   return output;
@@ -534,11 +542,11 @@ std::tuple<Tensor, Tensor, Tensor> beam_select_cuda(const Tensor& logits, const 
               "scores must be [batch, beams] on the logits' device");
   TORCH_CHECK(k >= 1 && k <= 64 && k <= beams * vocab, "k must be in 1 .. min(64, beams * vocab)");
   const c10::cuda::CUDAGuard guard(logits.device());
-  auto out_scores = at::empty({batch, k}, scores.options());
-  auto tokens = at::empty({batch, k}, scores.options().dtype(at::kInt));
-  auto parents = at::empty_like(tokens);
+  auto out_scores = fresh({batch, k}, at::kFloat, scores);
+  auto tokens = fresh({batch, k}, at::kInt, scores);
+  auto parents = fresh({batch, k}, at::kInt, scores);
   const size_t bytes = bc_beam_workspace_bytes(int(batch), int(beams), int(vocab), int(k));
-  auto workspace = at::empty({int64_t(bytes)}, scores.options().dtype(at::kByte));
+  auto workspace = fresh({int64_t(bytes)}, at::kByte, scores);
   const int dtype = logits.scalar_type() == at::kHalf       ? BC_F16
                     : logits.scalar_type() == at::kBFloat16 ? BC_BF16
                                                             : BC_F32;
@@ -557,10 +565,10 @@ std::tuple<Tensor, Tensor> run_beam_reorder(const Tensor& pages, const Tensor& l
                                             Tensor free_count_out, const char* op) {
   const int64_t batch = pages.size(0), beams = pages.size(1), width = pages.size(2),
                 out = parents.size(1);
-  auto pages_out = at::empty({batch, out, width}, pages.options());
-  auto lengths_out = at::empty({batch, out}, pages.options());
+  auto pages_out = fresh({batch, out, width}, at::kInt, pages);
+  auto lengths_out = fresh({batch, out}, at::kInt, pages);
   const size_t bytes = bc_reorder_workspace_bytes(int(batch), int(beams), int(width));
-  auto workspace = at::empty({int64_t(bytes)}, pages.options().dtype(at::kByte));
+  auto workspace = fresh({int64_t(bytes)}, at::kByte, pages);
   check_launch(bc_beam_reorder(int(batch), int(beams), int(out), int(refcount.numel()),
                                pages.data_ptr<int>(), int(width), lengths.data_ptr<int>(),
                                parents.data_ptr<int>(), refcount.data_ptr<int>(),
@@ -592,8 +600,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> beam_reorder_cuda(
     const Tensor& free_stack, const Tensor& free_count) {
   check_reorder(pages, lengths, parents, refcount, free_stack, free_count);
   const c10::cuda::CUDAGuard guard(pages.device());
-  auto refcount_out = at::empty_like(refcount), stack_out = at::empty_like(free_stack),
-       count_out = at::empty_like(free_count);
+  auto refcount_out = fresh(refcount.sizes(), at::kInt, pages),
+       stack_out = fresh(free_stack.sizes(), at::kInt, pages),
+       count_out = fresh(free_count.sizes(), at::kInt, pages);
   auto [po, lo] = run_beam_reorder(pages, lengths, parents, refcount, free_stack, free_count,
                                    refcount_out, stack_out, count_out, "beam_reorder");
   return {po, lo, refcount_out, stack_out, count_out};

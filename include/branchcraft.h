@@ -444,7 +444,8 @@ int bc_beam_select(int batch, int beams, int vocab, int k, int dtype, const void
  * the state may be its own input (an update in place). beams_in, beams_out at
  * most BC_MAX_BEAMS; no request's pages are held at two columns. Page ids
  * outside [0, P) set BC_ERR_PAGE_RANGE and are not counted. workspace:
- * bc_reorder_workspace_bytes, one per call in flight. Two launches. */
+ * bc_reorder_workspace_bytes, one per call in flight. Two launches, three with
+ * other arrays for the state. */
 size_t bc_reorder_workspace_bytes(int batch, int beams_in, int max_pages);
 int bc_beam_reorder(int batch, int beams_in, int beams_out, int physical_pages,
                     const int* pages_in, int max_pages, const int* lengths_in,
