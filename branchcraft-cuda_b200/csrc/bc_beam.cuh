@@ -17,8 +17,7 @@ constexpr int kBeamThreads = 256;
 constexpr int kBeamPerThread = 16;
 constexpr int kBeamTile = kBeamThreads * kBeamPerThread;  // logits of one step of a block
 constexpr int kBeamGroups = kBeamThreads / 2;             // two threads each
-constexpr int kBeamKeep = 512;                            // candidates before they are thinned
-constexpr int kBeamRoom = kBeamKeep + kBeamTile;          // and the most there can be
+constexpr int kBeamRoom = 2 * kBeamMaxK + 32 + kBeamTile;  // candidates there can be
 constexpr int kBeamThinned = kBeamMaxK * ((kBeamRoom + kBeamThreads - 1) / kBeamThreads);
 
 enum BeamType : int { kBeamF16 = 0, kBeamBF16 = 1, kBeamF32 = 2 };
@@ -186,6 +185,9 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const Bea
   float m = -INFINITY;
   double sum = 0.0;
   unsigned long long tau = 0;
+  // Candidates wait until there are twice k of them and some: a better bound lets
+  // fewer through, and a warp with one costs every lane its 16 comparisons.
+  const int keep = 2 * p.k + 32;
   __syncthreads();
   for (int w = w0; w < w1; w += kBeamTile) {
     if (w + kBeamTile < w1) load(w + kBeamTile, next);
@@ -236,14 +238,16 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const Bea
       tau = s_thin.tau;
     }
     bool full = false;
-    if (beam_order(mx) >= unsigned(tau >> 32)) {
+    const float bound = tau == 0 ? -INFINITY : beam_value(unsigned(tau >> 32));
+    if (mx >= bound) {
 #pragma unroll
       for (int j = 0; j < kBeamPerThread; ++j) {
+        if (!(v[j] >= bound)) continue;
         const unsigned long long key = key_of(j);
         if (key >= tau && key != 0) {
           const int i = atomicAdd(&s_n, 1);
           beam_cand[i] = key;
-          full = full || i >= kBeamKeep;
+          full = full || i >= keep;
           sum += double(expf(v[j] - base)) - double(fast_exp2((v[j] - base) * kLog2E));
         }
       }
