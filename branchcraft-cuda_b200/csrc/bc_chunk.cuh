@@ -22,8 +22,8 @@
 // not depend on timing.
 //
 // Warps: 0-3 and 4-7 softmax groups 0 and 1 (thread = row = TMEM lane), 8 the
-// scheduler (item descriptors, Q), 9 the issuer of S = Q K^T, 11 of O += P V, 10 the
-// K/V producer (a ring each, eight 16-row boxes a tile). TMEM holds one S (128
+// scheduler (item descriptors, Q) and V producer, 10 the K producer (a ring each,
+// eight 16-row boxes a tile), 9 the issuer of S = Q K^T, 11 of O += P V. TMEM holds one S (128
 // columns) that the groups use in turn, P of each group (64, 16-bit pairs) and O of
 // each (128). A group keeps S only while it loads its scores into registers, so the
 // next S, of the other group, is computed beside its exponentials, and a group's own
@@ -265,23 +265,6 @@ __device__ __forceinline__ void st_global_v8(void* to, uint32_t a, uint32_t b, u
                : "memory");
 }
 
-// The order of an item's copies: two K tiles first, then V and K in turn, then the
-// V tiles left over. The tile at place i:
-__device__ __forceinline__ int chunk_tile(int i, int nt, bool& is_v) {
-  const int lead = min(2, nt);
-  if (i < lead) {
-    is_v = false;
-    return i;
-  }
-  i -= lead;
-  if (i < 2 * (nt - lead)) {
-    is_v = (i & 1) == 0;
-    return is_v ? i >> 1 : (i >> 1) + lead;
-  }
-  is_v = true;
-  return i - (nt - lead);
-}
-
 // MOD: bit 0 the tanh cap, bit 1 the distance bias.
 template <int D, typename T, int MOD>
 __global__ void __launch_bounds__(kChThreads, 1)
@@ -399,8 +382,56 @@ __global__ void __launch_bounds__(kChThreads, 1)
   bool ok = true;
   if (warp >= 8) {
     regs_decrease<kChOtherRegs>();
+    // The copies of an item's K (or V) tiles, the warp's `tile0`-th on: lane l holds
+    // the page id of page (l & 7) of tile 4 batch + l / 8, loaded a batch ahead, and
+    // eight lanes issue a box each (a warp issues one per 70 ns or so: a producer
+    // each for K and V, since one for both held single-token calls to 57 GB/s a SM).
+    auto copy_tiles = [&](auto is_v, const ChunkDesc& d, unsigned tile0, unsigned& issued) -> bool {
+      constexpr bool V = decltype(is_v)::value;
+      constexpr int N = V ? NV : NK;
+      uint64_t *full = V ? v_full : k_full, *empty = V ? v_empty : k_empty;
+      const int* row = p.pages + size_t(d.request) * p.max_pages;
+      auto load_id = [&](int first) -> int {
+        const int j = first + (lane >> 3);
+        const int pg = (d.t0 + j) * (kChTile / kPageSize) + (lane & 7);
+        // pages that no row of the block sees stay out: the copy fills zeros
+        if (j >= d.nt || pg * kPageSize >= d.hi || (pg + 1) * kPageSize <= d.lo) return -1;
+        const int id = __ldg(row + pg);
+        if (id >= 0 && id < p.physical_pages) return id;
+        atomicOr(p.err, kErrPageRange);
+        return -1;
+      };
+      int cur = load_id(0), nxt = load_id(4);
+      for (int j = 0; j < d.nt; ++j) {
+        if (j > 0 && (j & 3) == 0) {
+          cur = nxt;
+          nxt = load_id(j + 4);
+        }
+        const unsigned s = tile0 + unsigned(j);
+        const int st = int(s % N);
+        if (s >= N && !__all_sync(0xffffffffu, mbar_wait(&empty[st], ((s / N) - 1) & 1))) return false;
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], uint32_t(G::kRowTile));
+        const int id = __shfl_sync(0xffffffffu, cur, (j & 3) * 8 + (lane & 7));
+        if (lane < 8)
+          tma_load_5d(tiles + G::kRingOff + ((V ? NK : 0) + st) * G::kRowTile + lane * G::kPageBytes,
+                      V ? &vmap : &kmap, &full[st], 0, 0, d.head * p.head_blocks, 0, id);
+        __syncwarp();
+        issued = s + 1;
+      }
+      return true;
+    };
+    // A failing launch waits out the copies in flight: the ring's last tiles.
+    auto drain_tiles = [&](auto is_v, unsigned issued) {
+      constexpr bool V = decltype(is_v)::value;
+      constexpr unsigned N = V ? NV : NK;
+      uint64_t* full = V ? v_full : k_full;
+      if (lane == 0)
+        for (unsigned s = issued - min(issued, N); s < issued; ++s)
+          mbar_drain(&full[s % N], (s / N) & 1);
+      __syncwarp();
+    };
     if (warp == 8) {
-      // ---------------------------------------------------------- scheduler
+      // ------------------------------------------- scheduler and V producer
       // This block's share: from its own cut (found by lanes 0-15) up to the next
       // block's (lanes 16-31). Cuts inside an item fall on multiples of `grain`
       // tiles from its start (a thirty-second of a share; at least kChMinPiece, half
@@ -526,9 +557,8 @@ __global__ void __launch_bounds__(kChThreads, 1)
       // (2) here, or this block has no share (3); and the item that starts here
       // and goes on
       int cont = left > 0 ? 0 : 3, has = 0, h_first = 0, h_ntok = 0, h_head = 0;
-      int k = 0;
-      bool q_pending = false;
-      for (;; ++k) {
+      // The piece at hand as a descriptor, handed to the other warps.
+      auto publish = [&](int k) -> ChunkDesc {
         ChunkDesc d = {};
         d.end = left <= 0;
         if (!d.end) {
@@ -557,13 +587,17 @@ __global__ void __launch_bounds__(kChThreads, 1)
         const int ds = k % kChDescs;
         if (k >= kChDescs)
           ok = __all_sync(0xffffffffu, mbar_wait(&desc_empty[ds], ((k / kChDescs) - 1) & 1));
-        if (!ok) break;
-        if (lane == 0) {
+        if (ok && lane == 0) {
           descs[ds] = d;
           mbar_arrive(&desc_full[ds]);
         }
         __syncwarp();
-        if (d.end) break;
+        return d;
+      };
+      ChunkDesc d = publish(0);
+      unsigned tile0 = 0, issued = 0;
+      int nq_loaded = 0;  // items whose Q has been asked for
+      for (int k = 0; ok && !d.end; ++k) {
         if (k > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_free, (k - 1) & 1));
         if (!ok) break;
         // Q of the block's row tiles; rows past the request's are other tokens'
@@ -577,13 +611,18 @@ __global__ void __launch_bounds__(kChThreads, 1)
                           kb * 64, d.head * p.group, d.first + i * p.tile_tokens);
         }
         __syncwarp();
-        q_pending = true;
+        nq_loaded = k + 1;
+        // the next piece is known before this one's V: K runs ahead
         if (off + d.nt < g.tiles) {  // the share ends inside this item
           left = 0;
         } else {
           next_item();
           left = mine_here();
         }
+        const ChunkDesc next = publish(k + 1);
+        if (ok) ok = copy_tiles(std::true_type{}, d, tile0, issued);
+        tile0 += unsigned(d.nt);
+        d = next;
       }
       if (p.sched && lane == 0) {
         int* s = p.sched + size_t(blockIdx.x) * 8;
@@ -593,7 +632,10 @@ __global__ void __launch_bounds__(kChThreads, 1)
         s[3] = h_ntok;
         s[4] = h_head;
       }
-      if (!ok && q_pending) mbar_drain(q_full, (k - (k > 0)) & 1);
+      if (!ok) {
+        if (nq_loaded > 0) mbar_drain(q_full, (nq_loaded - 1) & 1);
+        drain_tiles(std::true_type{}, issued);
+      }
     } else if (warp != 10) {
       // ------------------------------------------------------------ issuers
       // Warp 9: S_g = Q_g K^T, warp 11: O_g += P_g V, the groups in turn. (A
@@ -680,10 +722,8 @@ __global__ void __launch_bounds__(kChThreads, 1)
       if (lane == 0) mbar_drain(&fin[is_pv], 0);
       __syncwarp();
     } else {
-      // ----------------------------------------------------------- producer
-      // Lane l holds the page id of page (l & 7) of ring place 4 batch + l / 8,
-      // loaded a batch ahead.
-      unsigned tile0 = 0, k_next = 0, v_next = 0;  // first tile of the item; tiles issued
+      // --------------------------------------------------------- K producer
+      unsigned tile0 = 0, issued = 0;
       for (int k = 0; ok; ++k) {
         const int ds = k % kChDescs;
         ok = __all_sync(0xffffffffu, mbar_wait(&desc_full[ds], (k / kChDescs) & 1));
@@ -692,54 +732,10 @@ __global__ void __launch_bounds__(kChThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&desc_empty[ds]);
         if (d.end) break;
-        const int nt = d.nt, steps = 2 * nt;
-        const int* row = p.pages + size_t(d.request) * p.max_pages;
-        auto load_id = [&](int first) -> int {
-          const int i = first + (lane >> 3);
-          if (i >= steps) return -1;
-          bool is_v;
-          const int pg = (d.t0 + chunk_tile(i, nt, is_v)) * (kChTile / kPageSize) + (lane & 7);
-          // pages that no row of the block sees stay out: the copy fills zeros
-          if (pg * kPageSize >= d.hi || (pg + 1) * kPageSize <= d.lo) return -1;
-          const int id = __ldg(row + pg);
-          if (id < 0 || id >= p.physical_pages) {
-            atomicOr(p.err, kErrPageRange);
-            return -1;
-          }
-          return id;
-        };
-        int cur = load_id(0), nxt = load_id(4);
-        for (int i = 0; i < steps; ++i) {
-          if (i > 0 && (i & 3) == 0) {
-            cur = nxt;
-            nxt = load_id(i + 4);
-          }
-          bool is_v;
-          const unsigned s = tile0 + unsigned(chunk_tile(i, nt, is_v));
-          const int st = int(s % (is_v ? NV : NK));
-          uint64_t* full = (is_v ? v_full : k_full) + st;
-          if (s >= (is_v ? NV : NK))
-            ok = __all_sync(0xffffffffu, is_v ? mbar_wait(&v_empty[st], ((s / NV) - 1) & 1)
-                                              : mbar_wait(&k_empty[st], ((s / NK) - 1) & 1));
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(full, uint32_t(G::kRowTile));
-          const int id = __shfl_sync(0xffffffffu, cur, (i & 3) * 8 + (lane & 7));
-          if (lane < 8)
-            tma_load_5d(tiles + G::kRingOff + ((is_v ? NK : 0) + st) * G::kRowTile +
-                            lane * G::kPageBytes,
-                        is_v ? &vmap : &kmap, full, 0, 0, d.head * p.head_blocks, 0, id);
-          __syncwarp();
-          (is_v ? v_next : k_next) = s + 1;
-        }
-        tile0 += unsigned(nt);
+        ok = copy_tiles(std::false_type{}, d, tile0, issued);
+        tile0 += unsigned(d.nt);
       }
-      if (!ok && lane == 0) {  // copies in flight: each ring's last tiles
-        for (unsigned s = k_next - min(k_next, unsigned(NK)); s < k_next; ++s)
-          mbar_drain(&k_full[s % NK], (s / NK) & 1);
-        for (unsigned s = v_next - min(v_next, unsigned(NV)); s < v_next; ++s)
-          mbar_drain(&v_full[s % NV], (s / NV) & 1);
-      }
-      __syncwarp();
+      if (!ok) drain_tiles(std::false_type{}, issued);
     }
     if (!ok && lane == 0) atomicOr(p.err, kErrTimeout);
     tc_fence_before();
