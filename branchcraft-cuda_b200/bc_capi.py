@@ -103,7 +103,7 @@ _sigs = {
     "bc_chunk_workspace_bytes": [_SP, _i],
     "bc_chunk_attention": [_SP, _i, _i, _vp, _ll, _vp, _vp, _LP, _vp, _vp, _vp,
                            ctypes.POINTER(ChunkOptions), _vp, _i, _vp, _sz, _vp],
-    "bc_beam_workspace_bytes": [_i, _i, _i, _i],
+    "bc_beam_workspace_bytes": [_i, _i, _i, _i, _i],
     "bc_beam_select": [_i, _i, _i, _i, _i, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
     "bc_reorder_workspace_bytes": [_i, _i, _i],
     "bc_beam_reorder": [_i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
@@ -454,8 +454,8 @@ def chunk_attention(shape: Shape, q, cache_k, cache_v, pages, query_start, lengt
     return rc
 
 
-def beam_workspace_bytes(batch, beams, vocab, k) -> int:
-    return _lib.bc_beam_workspace_bytes(batch, beams, vocab, k)
+def beam_workspace_bytes(batch, beams, vocab, k, dtype) -> int:
+    return _lib.bc_beam_workspace_bytes(batch, beams, vocab, k, DTYPES[dtype])
 
 
 def beam_select(logits, scores, k, out_scores, out_tokens, out_parents, workspace, stream=None):

@@ -14,18 +14,77 @@ constexpr int kBeamMaxK = 64;     // pairs selected
 constexpr int kBeamMaxVocab = 1 << 20;
 constexpr int kBeamMergeThreads = 512;
 constexpr int kBeamThreads = 256;
-constexpr int kBeamPerThread = 16;
-constexpr int kBeamTile = kBeamThreads * kBeamPerThread;  // logits of one step of a block
-constexpr int kBeamGroups = kBeamThreads / 2;             // two threads each
-constexpr int kBeamRoom = 2 * kBeamMaxK + 32 + kBeamTile;  // candidates there can be
-constexpr int kBeamThinned = kBeamMaxK * ((kBeamRoom + kBeamThreads - 1) / kBeamThreads);
+constexpr int kBeamLoads = 4;                         // 16-byte loads of a thread's step
+constexpr int kBeamGroups = kBeamThreads / 2;         // two threads each
+
+// Logits of one step of a block, and the candidates there can be: those waiting
+// (2 k + 32 at most before they are thinned) and a whole step's.
+__host__ __device__ constexpr int beam_tile(int type_bytes) {
+  return kBeamThreads * kBeamLoads * (16 / type_bytes);
+}
+__host__ __device__ constexpr int beam_room(int type_bytes, int k) {
+  return 2 * k + 32 + beam_tile(type_bytes);
+}
+__host__ __device__ constexpr int beam_few(int type_bytes, int k) {  // thinned (beam_thin)
+  return k * ((beam_room(type_bytes, k) + kBeamThreads - 1) / kBeamThreads);
+}
 
 enum BeamType : int { kBeamF16 = 0, kBeamBF16 = 1, kBeamF32 = 2 };
 
-// A logit as the search sees it: NaN counts as -inf (never chosen before a
-// number), +inf as the largest number.
-__device__ __forceinline__ float beam_logit(float x) {
+// A score as the search sees it: NaN counts as -inf, +inf as the largest number.
+__device__ __forceinline__ float beam_score(float x) {
   return fminf(fmaxf(x, -INFINITY), 3.402823466e38f);
+}
+
+// Logits likewise (NaN is never chosen before a number, +inf is their type's
+// largest), two 16-bit ones at a time; and the larger of two words' logits.
+__device__ __forceinline__ uint32_t beam_clean(uint32_t x, const float*) {
+  return __float_as_uint(beam_score(__uint_as_float(x)));
+}
+__device__ __forceinline__ uint32_t beam_clean(uint32_t x, const __half*) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 t;\n\tmax.f16x2 t, %1, %2;\n\tmin.f16x2 %0, t, %3;\n\t}"
+      : "=r"(r) : "r"(x), "r"(0xfc00fc00u), "r"(0x7bff7bffu));
+  return r;
+}
+__device__ __forceinline__ uint32_t beam_clean(uint32_t x, const __nv_bfloat16*) {
+  uint32_t r;
+  asm("{\n\t.reg .b32 t;\n\tmax.bf16x2 t, %1, %2;\n\tmin.bf16x2 %0, t, %3;\n\t}"
+      : "=r"(r) : "r"(x), "r"(0xff80ff80u), "r"(0x7f7f7f7fu));
+  return r;
+}
+__device__ __forceinline__ uint32_t beam_max(uint32_t x, uint32_t y, const float*) {
+  return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
+}
+__device__ __forceinline__ uint32_t beam_max(uint32_t x, uint32_t y, const __half*) {
+  uint32_t r;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  return r;
+}
+__device__ __forceinline__ uint32_t beam_max(uint32_t x, uint32_t y, const __nv_bfloat16*) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  return r;
+}
+// Logit i of a word.
+__device__ __forceinline__ float beam_float(uint32_t w, int, const float*) { return __uint_as_float(w); }
+__device__ __forceinline__ float beam_float(uint32_t w, int i, const __half*) {
+  const float2 f = unpack_half2(w);
+  return i ? f.y : f.x;
+}
+__device__ __forceinline__ float beam_float(uint32_t w, int i, const __nv_bfloat16*) {
+  return __uint_as_float(i ? w & 0xffff0000u : w << 16);
+}
+
+__device__ __forceinline__ float beam_one(float x) { return beam_score(x); }
+__device__ __forceinline__ float beam_one(__half x) {
+  return beam_float(beam_clean(uint32_t(__half_as_ushort(x)), static_cast<const __half*>(nullptr)), 0,
+                    static_cast<const __half*>(nullptr));
+}
+__device__ __forceinline__ float beam_one(__nv_bfloat16 x) {
+  return beam_float(
+      beam_clean(uint32_t(__bfloat16_as_ushort(x)), static_cast<const __nv_bfloat16*>(nullptr)), 0,
+      static_cast<const __nv_bfloat16*>(nullptr));
 }
 
 // Keys: larger value first, then the lower index. Unique, so selection never
@@ -50,7 +109,7 @@ __device__ __forceinline__ double beam_value64(unsigned long long u) {
 
 struct BeamSelectParams {
   int batch, beams, vocab, k;
-  int segments, segment;  // blocks of a row, their steps' logits (a multiple of kBeamTile)
+  int segments, segment;  // blocks of a row, their steps' logits (a multiple of the step)
   const void* logits;
   long long row_stride;  // elements between two beams' rows
   const float* scores;   // [batch, beams]
@@ -63,26 +122,6 @@ struct BeamSelectParams {
   float* seg_max;            // [rows, segments]
   double* seg_sum;           // [rows, segments]
 };
-
-template <typename T>
-struct BeamRaw {  // a thread's logits of one step as loaded
-  static constexpr int kVec = 16 / int(sizeof(T));
-  static constexpr int kLoads = kBeamPerThread / kVec;
-  uint4 v[kLoads];
-};
-
-__device__ __forceinline__ float beam_float(const uint4& v, int i, float*) {
-  return __uint_as_float(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
-}
-__device__ __forceinline__ float beam_float(const uint4& v, int i, __half*) {
-  const uint32_t w = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
-  const float2 f = unpack_half2(w);
-  return (i & 1) ? f.y : f.x;
-}
-__device__ __forceinline__ float beam_float(const uint4& v, int i, __nv_bfloat16*) {
-  const uint32_t w = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
-  return __uint_as_float((i & 1) ? w & 0xffff0000u : w << 16);
-}
 
 // What the thinning of candidates needs beside them.
 struct BeamThin {
@@ -132,7 +171,7 @@ __device__ __noinline__ int beam_thin(unsigned long long* cand, unsigned long lo
   return n;
 }
 
-// One block per segment of a row, a step of kBeamTile logits at a time, the next
+// One block per segment of a row, a step of four loads a thread at a time, the next
 // step's loads in flight. HBM bound: each logit is read once (16-byte loads where
 // a vector lies inside the row), compared with the k-th best so far, and added to
 // its thread's sum under the thread's own running maximum. The first step's bound
@@ -141,13 +180,14 @@ __device__ __noinline__ int beam_thin(unsigned long long* cand, unsigned long lo
 // The sum takes ex2.approx (relative error 2^-22 and that of the argument, two
 // roundings); logits that pass the bound, the ones that weigh, are put right by
 // expf, since the order of two beams' candidates hangs on the last digits; a
-// thread's 16 terms of a step are added in FP32, the steps in 64 bits.
+// thread's 16 or 32 terms of a step are added in FP32, the steps in 64 bits.
 template <typename T>
-__global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const BeamSelectParams p) {
-  using Raw = BeamRaw<T>;
+__global__ void __launch_bounds__(kBeamThreads, 3) beam_segment_kernel(const BeamSelectParams p) {
   constexpr float kLog2E = 1.4426950408889634f;
-  constexpr int VEC = Raw::kVec;
-  extern __shared__ unsigned long long beam_cand[];  // [kBeamRoom], then [kBeamThinned]
+  // a thread's logits of a step: 16 words, PW to a word, VEC to a load
+  constexpr int PW = 4 / int(sizeof(T)), VEC = 4 * PW, PT = VEC * kBeamLoads, TILE = beam_tile(sizeof(T));
+  constexpr const T* kType = nullptr;
+  extern __shared__ unsigned long long beam_cand[];  // [beam_room], then [beam_few]
   __shared__ BeamThin s_thin;
   __shared__ float s_max[kBeamThreads / 32];
   __shared__ double s_sum[kBeamThreads / 32];
@@ -165,22 +205,27 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const Bea
   const int mis = int((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const T* x0 = x - mis;
   const int w0 = seg * p.segment, w1 = min(w0 + p.segment, p.vocab + mis);
-  auto load = [&](int w, Raw& raw) {
+  auto load = [&](int w, uint32_t (&raw)[16]) {
 #pragma unroll
-    for (int j = 0; j < Raw::kLoads; ++j) {
+    for (int j = 0; j < kBeamLoads; ++j) {
       const int at = w + (j * kBeamThreads + tid) * VEC;
+      uint4 v;
       if (at >= mis && at + VEC <= p.vocab + mis) {
-        raw.v[j] = __ldcs(reinterpret_cast<const uint4*>(x0 + at));
+        v = __ldcs(reinterpret_cast<const uint4*>(x0 + at));
       } else {  // a vector across the row's ends: its own logits alone
         T e[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
           e[i] = at + i >= mis && at + i < p.vocab + mis ? x0[at + i] : T(-INFINITY);
-        raw.v[j] = *reinterpret_cast<const uint4*>(e);
+        v = *reinterpret_cast<const uint4*>(e);
       }
+      raw[4 * j] = v.x;
+      raw[4 * j + 1] = v.y;
+      raw[4 * j + 2] = v.z;
+      raw[4 * j + 3] = v.w;
     }
   };
-  Raw raw, next;
+  uint32_t raw[16], next[16];
   if (w0 < w1) load(w0, raw);
   float m = -INFINITY;
   double sum = 0.0;
@@ -189,20 +234,28 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const Bea
   // fewer through, and a warp with one costs every lane its 16 comparisons.
   const int keep = 2 * p.k + 32;
   __syncthreads();
-  for (int w = w0; w < w1; w += kBeamTile) {
-    if (w + kBeamTile < w1) load(w + kBeamTile, next);
-    float v[kBeamPerThread];
-    float mx = -INFINITY;
+  for (int w = w0; w < w1; w += TILE) {
+    if (w + TILE < w1) load(w + TILE, next);
 #pragma unroll
-    for (int j = 0; j < kBeamPerThread; ++j) {
-      v[j] = beam_logit(beam_float(raw.v[j / VEC], j % VEC, static_cast<T*>(nullptr)));
-      mx = fmaxf(mx, v[j]);
+    for (int i = 0; i < 16; ++i) raw[i] = beam_clean(raw[i], kType);
+    auto val = [&](int j) { return beam_float(raw[j / PW], j % PW, kType); };
+    float mx;
+    {
+      uint32_t big = raw[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) big = beam_max(big, raw[i], kType);
+      mx = fmaxf(beam_float(big, 0, kType), beam_float(big, PW - 1, kType));
     }
-    auto place = [&](int j) { return w + (j / VEC * kBeamThreads + tid) * VEC + j % VEC; };
-    auto key_of = [&](int j) -> unsigned long long {  // 0: no logit of the row
-      const int at = place(j);
-      return at >= mis && at < w1 ? beam_key(v[j], unsigned(at - mis)) : 0ull;
+    // the thread's logits at or above `bound`, a bit each (its last bits: the first
+    // logits), those of other rows left out
+    auto at_or_above = [&](float bound) -> uint32_t {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int j = 0; j < PT; ++j) bits |= val(j) >= bound ? 1u << j : 0u;
+      return bits;
     };
+    auto place = [&](int j) { return w + (j / VEC * kBeamThreads + tid) * VEC + j % VEC; };
+    auto in_row = [&](int j) { return place(j) >= mis && place(j) < w1; };
     if (mx > m) {  // the thread's sum follows its running maximum
       sum *= double(expf(m - mx));
       m = mx;
@@ -210,18 +263,20 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const Bea
     const float base = m == -INFINITY ? 0.f : m;
     uint64_t e = 0;  // (two zeros)
 #pragma unroll
-    for (int j = 0; j < kBeamPerThread; j += 2) {
-      const float2 d = pair_floats(mul2(add2(pair_of(v[j], v[j + 1]), pair_of(-base, -base)),
+    for (int j = 0; j < PT; j += 2) {
+      const float2 d = pair_floats(mul2(add2(pair_of(val(j), val(j + 1)), pair_of(-base, -base)),
                                         pair_of(kLog2E, kLog2E)));
       e = add2(e, pair_of(fast_exp2(d.x), fast_exp2(d.y)));
     }
     sum += double(pair_floats(e).x + pair_floats(e).y);
     if (w == w0) {
       unsigned long long best = 0;
-#pragma unroll
-      for (int j = 0; j < kBeamPerThread; ++j) {
-        const unsigned long long key = v[j] == mx ? key_of(j) : 0ull;
-        best = key > best ? key : best;
+      for (uint32_t bits = at_or_above(mx); bits; bits &= bits - 1) {
+        const int j = __ffs(bits) - 1;
+        if (in_row(j)) {
+          best = beam_key(mx, unsigned(place(j) - mis));
+          break;
+        }
       }
       const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, 1);
       best = other > best ? other : best;
@@ -240,27 +295,29 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const Bea
     bool full = false;
     const float bound = tau == 0 ? -INFINITY : beam_value(unsigned(tau >> 32));
     if (mx >= bound) {
-#pragma unroll
-      for (int j = 0; j < kBeamPerThread; ++j) {
-        if (!(v[j] >= bound)) continue;
-        const unsigned long long key = key_of(j);
-        if (key >= tau && key != 0) {
-          const int i = atomicAdd(&s_n, 1);
-          beam_cand[i] = key;
-          full = full || i >= keep;
-          sum += double(expf(v[j] - base)) - double(fast_exp2((v[j] - base) * kLog2E));
-        }
+      for (uint32_t bits = at_or_above(bound); bits; bits &= bits - 1) {
+        const int j = __ffs(bits) - 1;
+        if (!in_row(j)) continue;
+        // (few: read again, rather than picked out of the registers)
+        const float v = beam_one(x0[place(j)]);
+        const unsigned long long key = beam_key(v, unsigned(place(j) - mis));
+        if (key < tau) continue;
+        const int i = atomicAdd(&s_n, 1);
+        beam_cand[i] = key;
+        full = full || i >= keep;
+        sum += double(expf(v - base)) - double(fast_exp2((v - base) * kLog2E));
       }
     }
     // (the answer has to be the block's: s_n may have moved on for some)
     full = __syncthreads_or(full);
-    if (full || w + kBeamTile >= w1) {
-      const int kept = beam_thin(beam_cand, beam_cand + kBeamRoom, s_thin, s_n, p.k);
+    if (full || w + TILE >= w1) {
+      const int kept = beam_thin(beam_cand, beam_cand + beam_room(sizeof(T), p.k), s_thin, s_n, p.k);
       if (kept == p.k) tau = beam_cand[kept - 1] + 1;  // only better ones from now on
       if (tid == 0) s_n = kept;
       __syncthreads();
     }
-    raw = next;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) raw[i] = next[i];
   }
   const size_t at = size_t(blockIdx.x) * p.k;
   const int kept = w0 < w1 ? min(s_n, p.k) : 0;
@@ -319,7 +376,7 @@ __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const Bea
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
     // a row without a possible token, and a beam that is out, give -inf
-    const float score = beam_logit(p.scores[size_t(b) * p.beams + w]);
+    const float score = beam_score(p.scores[size_t(b) * p.beams + w]);
     if (lane == 0) {
       s_off[w] = m == -INFINITY || score == -INFINITY ? -INFINITY : double(score) - log(s);
       s_top[w] = m == -INFINITY ? 0.f : m;

@@ -1177,24 +1177,25 @@ cudaError_t launch_chunk(ChunkParams& p, const CUtensorMap* maps, const ChunkPla
 }
 
 // Rows are cut into the number of segments that takes the least time by count:
-// waves of four blocks a SM times a segment's steps and its fixed work (the first
-// bound and the last ranking, some four steps' time).
+// waves of three blocks a SM times a segment's steps and its fixed work (the first
+// bound and the last ranking, some three steps' time).
 struct BeamPlan {
   int segments, segment;
-  BeamPlan(int rows, int vocab, int dev) {
-    const int steps = (vocab + 15 + kBeamTile - 1) / kBeamTile;  // (from a 16-byte boundary on)
-    const long long slots = 4ll * (dev < 0 ? 148 : sm_count(dev));
+  BeamPlan(int rows, int vocab, int type_bytes, int dev) {
+    const int tile = beam_tile(type_bytes);
+    const int steps = (vocab + 15 + tile - 1) / tile;  // (from a 16-byte boundary on)
+    const long long slots = 3ll * (dev < 0 ? 148 : sm_count(dev));
     long long least = -1;
     int per = steps;
     for (int s = 1; s <= steps && (s == 1 || (long long)rows * s <= 4 * slots); ++s) {
       const int each = (steps + s - 1) / s;
-      const long long time = (((long long)rows * s + slots - 1) / slots) * (each + 4);
+      const long long time = (((long long)rows * s + slots - 1) / slots) * (each + 3);
       if (least < 0 || time < least) {
         least = time;
         per = each;
       }
     }
-    segment = per * kBeamTile;
+    segment = per * tile;
     segments = (vocab + 15 + segment - 1) / segment;
   }
 };
@@ -1202,11 +1203,17 @@ struct BeamPlan {
 template <typename T>
 cudaError_t launch_beam_segments(const BeamSelectParams& p, int dev, cudaStream_t stream) {
   static std::atomic<uint64_t> configured{0};
-  constexpr size_t smem = size_t(kBeamRoom + kBeamThinned) * 8;
-  const cudaError_t e = raise_smem(beam_segment_kernel<T>, smem, configured, dev);
+  const auto smem = [](int k) {
+    return size_t(beam_room(sizeof(T), k) + beam_few(sizeof(T), k)) * 8;
+  };
+  const cudaError_t e = raise_smem(beam_segment_kernel<T>, smem(kBeamMaxK), configured, dev);
   if (e != cudaSuccess) return e;
   return launch_dependent(beam_segment_kernel<T>, dim3(unsigned(p.batch) * p.beams * p.segments),
-                          kBeamThreads, smem, stream, p);
+                          kBeamThreads, smem(p.k), stream, p);
+}
+
+int beam_type_bytes(int dtype) {
+  return dtype == BC_F32 ? 4 : dtype == BC_F16 || dtype == BC_BF16 ? 2 : 0;
 }
 
 size_t beam_merge_smem(long long lists, int k) {
@@ -1378,10 +1385,10 @@ int bc_chunk_attention(const bc_shape* s, int tokens, int dtype, const void* q,
                          : launch_chunk<128, __nv_bfloat16>(p, maps, plan, options, dev, st);
 }
 
-size_t bc_beam_workspace_bytes(int batch, int beams, int vocab, int k) {
-  if (!beam_shape_ok(batch, beams, vocab, k)) return 0;
+size_t bc_beam_workspace_bytes(int batch, int beams, int vocab, int k, int dtype) {
+  if (!beam_shape_ok(batch, beams, vocab, k) || beam_type_bytes(dtype) == 0) return 0;
   // per segment: k keys, its sum and its largest logit
-  const BeamPlan plan(batch * beams, vocab, current_device());
+  const BeamPlan plan(batch * beams, vocab, beam_type_bytes(dtype), current_device());
   return size_t(batch) * beams * plan.segments * (size_t(k) * 8 + 8 + 4);
 }
 
@@ -1389,11 +1396,11 @@ int bc_beam_select(int batch, int beams, int vocab, int k, int dtype, const void
                    long long row_stride, const float* scores, float* out_scores, int* out_tokens,
                    int* out_parents, void* workspace, size_t workspace_bytes, void* stream) {
   if (!beam_shape_ok(batch, beams, vocab, k) ||
-      (dtype != BC_F16 && dtype != BC_BF16 && dtype != BC_F32) || !logits || row_stride < vocab ||
+      beam_type_bytes(dtype) == 0 || !logits || row_stride < vocab ||
       !scores || !out_scores || !out_tokens || !out_parents || !workspace ||
       address_bits(workspace) % 16 ||
-      address_bits(logits) % (dtype == BC_F32 ? 4 : 2) ||
-      workspace_bytes < bc_beam_workspace_bytes(batch, beams, vocab, k))
+      address_bits(logits) % beam_type_bytes(dtype) ||
+      workspace_bytes < bc_beam_workspace_bytes(batch, beams, vocab, k, dtype))
     return cudaErrorInvalidValue;
   const int dev = current_device();
   if (dev < 0) return cudaErrorInvalidDevice;
@@ -1402,7 +1409,7 @@ int bc_beam_select(int batch, int beams, int vocab, int k, int dtype, const void
   p.beams = beams;
   p.vocab = vocab;
   p.k = k;
-  const BeamPlan plan(batch * beams, vocab, dev);
+  const BeamPlan plan(batch * beams, vocab, beam_type_bytes(dtype), dev);
   p.segments = plan.segments;
   p.segment = plan.segment;
   p.logits = logits;
@@ -1421,8 +1428,8 @@ int bc_beam_select(int batch, int beams, int vocab, int k, int dtype, const void
                                      : launch_beam_segments<float>(p, dev, st);
   if (e != cudaSuccess) return e;
   static std::atomic<uint64_t> configured{0};
-  // (a request's lists: at most sixteen blocks a SM, or one a beam)
-  e = raise_smem(beam_merge_kernel, beam_merge_smem(std::max(16 * sm_count(dev), kBeamMax), kBeamMaxK),
+  // (a request's lists: at most twelve blocks a SM, or one a beam)
+  e = raise_smem(beam_merge_kernel, beam_merge_smem(std::max(12 * sm_count(dev), kBeamMax), kBeamMaxK),
                  configured, dev);
   if (e != cudaSuccess) return e;
   return launch_dependent(beam_merge_kernel, dim3(unsigned(batch)), kBeamMergeThreads,

@@ -545,11 +545,11 @@ std::tuple<Tensor, Tensor, Tensor> beam_select_cuda(const Tensor& logits, const 
   auto out_scores = fresh({batch, k}, at::kFloat, scores);
   auto tokens = fresh({batch, k}, at::kInt, scores);
   auto parents = fresh({batch, k}, at::kInt, scores);
-  const size_t bytes = bc_beam_workspace_bytes(int(batch), int(beams), int(vocab), int(k));
-  auto workspace = fresh({int64_t(bytes)}, at::kByte, scores);
   const int dtype = logits.scalar_type() == at::kHalf       ? BC_F16
                     : logits.scalar_type() == at::kBFloat16 ? BC_BF16
                                                             : BC_F32;
+  const size_t bytes = bc_beam_workspace_bytes(int(batch), int(beams), int(vocab), int(k), dtype);
+  auto workspace = fresh({int64_t(bytes)}, at::kByte, scores);
   check_launch(bc_beam_select(int(batch), int(beams), int(vocab), int(k), dtype,
                               logits.data_ptr(), row_stride, scores.data_ptr<float>(),
                               out_scores.data_ptr<float>(), tokens.data_ptr<int>(),

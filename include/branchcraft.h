@@ -420,14 +420,14 @@ int bc_chunk_attention(const bc_shape* shape, int tokens, int dtype, const void*
  * scores[b, w] + logits[b, w, v] - log(sum_u exp logits[b, w, u]), the largest
  * first, equal ones by the lowest w*vocab + v. logits [batch*beams, vocab] of
  * `dtype` (BC_F16, BC_BF16, BC_F32), row_stride elements between rows; scores
- * [batch, beams] FP32. A NaN logit counts as -inf and +inf as the largest
- * number; a beam whose score is -inf or NaN, or all of whose logits are -inf,
+ * [batch, beams] FP32. A NaN logit counts as -inf and +inf as its type's
+ * largest number; a beam whose score is -inf or NaN, or all of whose logits are -inf,
  * gives -inf. Written, [batch, k]: out_scores FP32, out_tokens, out_parents (the
  * beam). 1 <= k <= min(64, beams*vocab), beams at most 64, vocab at most 2^20.
  * workspace: bc_beam_workspace_bytes, 16-byte aligned, one per call in flight. */
 #define BC_MAX_BEAMS 64
 #define BC_MAX_BEAM_VOCAB (1 << 20)
-size_t bc_beam_workspace_bytes(int batch, int beams, int vocab, int k);
+size_t bc_beam_workspace_bytes(int batch, int beams, int vocab, int k, int dtype);
 int bc_beam_select(int batch, int beams, int vocab, int k, int dtype, const void* logits,
                    long long row_stride, const float* scores, float* out_scores,
                    int* out_tokens, int* out_parents, void* workspace, size_t workspace_bytes,

@@ -159,7 +159,7 @@ def assert_chunk_close(got, want, dtype, out_dtype=None):
 def beam_scores(logits, scores):
     """[batch, beams, vocab] float64 candidates."""
     x = logits.detach().cpu().double()
-    x = torch.where(torch.isnan(x), -math.inf, x).clamp(max=float(torch.finfo(torch.float32).max))
+    x = torch.where(torch.isnan(x), -math.inf, x).clamp(max=float(torch.finfo(logits.dtype).max))
     m = x.amax(-1, keepdim=True)
     safe = torch.where(m == -math.inf, 0.0, m)
     total = torch.exp(x - safe).sum(-1, keepdim=True).log()

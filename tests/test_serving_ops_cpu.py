@@ -102,7 +102,7 @@ def test_chunk_refusals():
 def test_beam_refusals():
     def call(batch=2, beams=3, vocab=50, k=4, dtype=2, logits=P, stride=50, ws=P, size=None):
         if size is None:
-            size = C.beam_workspace_bytes(batch, beams, vocab, k)
+            size = LIB.bc_beam_workspace_bytes(batch, beams, vocab, k, dtype)
         return LIB.bc_beam_select(batch, beams, vocab, k, dtype, logits, stride, P, P, P, P, ws,
                                   size, None)
 
@@ -111,8 +111,8 @@ def test_beam_refusals():
                dict(dtype=3), dict(dtype=-1), dict(logits=None), dict(logits=ODD),
                dict(stride=49), dict(ws=None), dict(ws=ODD), dict(size=10)):
         assert call(**kw) == 1, kw
-    assert C.beam_workspace_bytes(2, 3, 50, 65) == 0
-    assert C.beam_workspace_bytes(2, 3, 50, 4) > 0
+    assert C.beam_workspace_bytes(2, 3, 50, 65, torch.float32) == 0
+    assert C.beam_workspace_bytes(2, 3, 50, 4, torch.float32) > 0
 
 
 def test_reorder_refusals():
