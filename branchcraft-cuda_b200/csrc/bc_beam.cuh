@@ -17,16 +17,19 @@ constexpr int kBeamThreads = 256;
 constexpr int kBeamLoads = 4;                         // 16-byte loads of a thread's step
 constexpr int kBeamGroups = kBeamThreads / 2;         // two threads each
 
-// Logits of one step of a block, and the candidates there can be: those waiting
-// (2 k + 32 at most before they are thinned) and a whole step's.
+constexpr int kBeamSteps = 16;  // steps whose threads' maxima are kept
+
+// Logits of one step of a block; the candidates there can be: those waiting (2 k +
+// 32 at most before they are thinned) and those of one load by all threads.
 __host__ __device__ constexpr int beam_tile(int type_bytes) {
   return kBeamThreads * kBeamLoads * (16 / type_bytes);
 }
-__host__ __device__ constexpr int beam_room(int type_bytes, int k) {
-  return 2 * k + 32 + beam_tile(type_bytes);
+__host__ __device__ constexpr int beam_room(int k) { return 2 * k + 32 + kBeamThreads * 8; }
+__host__ __device__ constexpr int beam_few(int k) {  // thinned (beam_thin)
+  return k * ((beam_room(k) + kBeamThreads - 1) / kBeamThreads);
 }
-__host__ __device__ constexpr int beam_few(int type_bytes, int k) {  // thinned (beam_thin)
-  return k * ((beam_room(type_bytes, k) + kBeamThreads - 1) / kBeamThreads);
+__host__ __device__ constexpr size_t beam_smem(int k) {
+  return size_t(beam_room(k) + beam_few(k)) * 8 + size_t(kBeamSteps) * kBeamThreads * 4;
 }
 
 enum BeamType : int { kBeamF16 = 0, kBeamBF16 = 1, kBeamF32 = 2 };
@@ -171,23 +174,24 @@ __device__ __noinline__ int beam_thin(unsigned long long* cand, unsigned long lo
   return n;
 }
 
-// One block per segment of a row, a step of four loads a thread at a time, the next
-// step's loads in flight. HBM bound: each logit is read once (16-byte loads where
-// a vector lies inside the row), compared with the k-th best so far, and added to
-// its thread's sum under the thread's own running maximum. The first step's bound
-// is the k-th largest of 128 groups' maxima (the segment's k best lie in k groups);
-// after it few logits pass, and passing ones wait in shared memory to be thinned.
-// The sum takes ex2.approx (relative error 2^-22 and that of the argument, two
-// roundings); logits that pass the bound, the ones that weigh, are put right by
-// expf, since the order of two beams' candidates hangs on the last digits; a
-// thread's 16 or 32 terms of a step are added in FP32, the steps in 64 bits.
+// One block per segment of a row. HBM bound: one pass of 16-byte loads, the next
+// step's in flight, in which every thread keeps its largest logit (the first such)
+// and its sum of exp(x - largest) under its running maximum, no barrier between the
+// steps. The k-th largest of 128 thread pairs' best keys bounds the segment's k best,
+// which lie in k pairs: those few threads look again (from L2) at the steps whose
+// maxima, kept in shared memory, reach the bound and list what passes. Should the
+// list run over, they go through all steps a load at a time, thinning it on the way.
+// The sum takes ex2.approx of (x - largest) log2(e): relative error 2^-22 and the
+// argument's, none for the thread's largest logit itself; a step's 16 or 32 terms are
+// added in FP32, the steps and threads in 64 bits, since the order of two beams'
+// candidates hangs on the last digits.
 template <typename T>
-__global__ void __launch_bounds__(kBeamThreads, 3) beam_segment_kernel(const BeamSelectParams p) {
+__global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const BeamSelectParams p) {
   constexpr float kLog2E = 1.4426950408889634f;
   // a thread's logits of a step: 16 words, PW to a word, VEC to a load
   constexpr int PW = 4 / int(sizeof(T)), VEC = 4 * PW, PT = VEC * kBeamLoads, TILE = beam_tile(sizeof(T));
   constexpr const T* kType = nullptr;
-  extern __shared__ unsigned long long beam_cand[];  // [beam_room], then [beam_few]
+  extern __shared__ unsigned long long beam_cand[];  // [beam_room], [beam_few], step maxima
   __shared__ BeamThin s_thin;
   __shared__ float s_max[kBeamThreads / 32];
   __shared__ double s_sum[kBeamThreads / 32];
@@ -227,38 +231,37 @@ __global__ void __launch_bounds__(kBeamThreads, 3) beam_segment_kernel(const Bea
   };
   uint32_t raw[16], next[16];
   if (w0 < w1) load(w0, raw);
-  float m = -INFINITY;
-  double sum = 0.0;
-  unsigned long long tau = 0;
-  // Candidates wait until there are twice k of them and some: a better bound lets
-  // fewer through, and a warp with one costs every lane its 16 comparisons.
-  const int keep = 2 * p.k + 32;
-  __syncthreads();
-  for (int w = w0; w < w1; w += TILE) {
-    if (w + TILE < w1) load(w + TILE, next);
+  auto val = [&](int j) { return beam_float(raw[j / PW], j % PW, kType); };
+  // the thread's logits at or above `bound`, a bit each
+  auto at_or_above = [&](float bound) -> uint32_t {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < PT; ++j) bits |= val(j) >= bound ? 1u << j : 0u;
+    return bits;
+  };
+  auto clean = [&]() -> float {  // raw made ready; its largest logit
 #pragma unroll
     for (int i = 0; i < 16; ++i) raw[i] = beam_clean(raw[i], kType);
-    auto val = [&](int j) { return beam_float(raw[j / PW], j % PW, kType); };
-    float mx;
-    {
-      uint32_t big = raw[0];
+    uint32_t big = raw[0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) big = beam_max(big, raw[i], kType);
-      mx = fmaxf(beam_float(big, 0, kType), beam_float(big, PW - 1, kType));
-    }
-    // the thread's logits at or above `bound`, a bit each (its last bits: the first
-    // logits), those of other rows left out
-    auto at_or_above = [&](float bound) -> uint32_t {
-      uint32_t bits = 0;
-#pragma unroll
-      for (int j = 0; j < PT; ++j) bits |= val(j) >= bound ? 1u << j : 0u;
-      return bits;
-    };
-    auto place = [&](int j) { return w + (j / VEC * kBeamThreads + tid) * VEC + j % VEC; };
-    auto in_row = [&](int j) { return place(j) >= mis && place(j) < w1; };
-    if (mx > m) {  // the thread's sum follows its running maximum
-      sum *= double(expf(m - mx));
+    for (int i = 1; i < 16; ++i) big = beam_max(big, raw[i], kType);
+    return fmaxf(beam_float(big, 0, kType), beam_float(big, PW - 1, kType));
+  };
+  auto place = [&](int w, int j) { return w + (j / VEC * kBeamThreads + tid) * VEC + j % VEC; };
+  const int room = beam_room(p.k);
+  unsigned long long* few = beam_cand + room;
+  float* step_max = reinterpret_cast<float*>(few + beam_few(p.k)) + tid;  // [step * kBeamThreads]
+  float m = -INFINITY;
+  double sum = 0.0;
+  int top = w0;  // the first step with the largest logit
+  for (int w = w0, i = 0; w < w1; w += TILE, ++i) {
+    if (w + TILE < w1) load(w + TILE, next);
+    const float mx = clean();
+    if (i < kBeamSteps) step_max[i * kBeamThreads] = mx;
+    if (mx > m) {
+      sum *= m == -INFINITY ? 0.0 : double(expf(m - mx));
       m = mx;
+      top = w;
     }
     const float base = m == -INFINITY ? 0.f : m;
     uint64_t e = 0;  // (two zeros)
@@ -269,59 +272,87 @@ __global__ void __launch_bounds__(kBeamThreads, 3) beam_segment_kernel(const Bea
       e = add2(e, pair_of(fast_exp2(d.x), fast_exp2(d.y)));
     }
     sum += double(pair_floats(e).x + pair_floats(e).y);
-    if (w == w0) {
-      unsigned long long best = 0;
-      for (uint32_t bits = at_or_above(mx); bits; bits &= bits - 1) {
-        const int j = __ffs(bits) - 1;
-        if (in_row(j)) {
-          best = beam_key(mx, unsigned(place(j) - mis));
-          break;
-        }
-      }
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, 1);
-      best = other > best ? other : best;
-      s_thin.best[tid] = best;
-      __syncthreads();
-      // both threads of a group count against half the groups
-      int above = 0;
-#pragma unroll 8
-      for (int i = 0; i < kBeamGroups / 2; ++i)
-        above += s_thin.best[((tid & 1) * (kBeamGroups / 2) + i) * 2] > best;
-      above += __shfl_xor_sync(0xffffffffu, above, 1);
-      if (above == p.k - 1 && best != 0 && (tid & 1) == 0) s_thin.tau = best;
-      __syncthreads();
-      tau = s_thin.tau;
-    }
-    bool full = false;
-    const float bound = tau == 0 ? -INFINITY : beam_value(unsigned(tau >> 32));
-    if (mx >= bound) {
-      for (uint32_t bits = at_or_above(bound); bits; bits &= bits - 1) {
-        const int j = __ffs(bits) - 1;
-        if (!in_row(j)) continue;
-        // (few: read again, rather than picked out of the registers)
-        const float v = beam_one(x0[place(j)]);
-        const unsigned long long key = beam_key(v, unsigned(place(j) - mis));
-        if (key < tau) continue;
-        const int i = atomicAdd(&s_n, 1);
-        beam_cand[i] = key;
-        full = full || i >= keep;
-        sum += double(expf(v - base)) - double(fast_exp2((v - base) * kLog2E));
-      }
-    }
-    // (the answer has to be the block's: s_n may have moved on for some)
-    full = __syncthreads_or(full);
-    if (full || w + TILE >= w1) {
-      const int kept = beam_thin(beam_cand, beam_cand + beam_room(sizeof(T), p.k), s_thin, s_n, p.k);
-      if (kept == p.k) tau = beam_cand[kept - 1] + 1;  // only better ones from now on
-      if (tid == 0) s_n = kept;
-      __syncthreads();
-    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) raw[i] = next[i];
   }
+  // the thread's best key (0: it has no logit of the row)
+  unsigned long long best = 0;
+  for (int w = top; w < w1 && best == 0; w += TILE) {
+    load(w, raw);
+    clean();
+    for (uint32_t bits = at_or_above(m); bits; bits &= bits - 1) {
+      const int at = place(w, __ffs(bits) - 1);
+      if (at >= mis && at < w1) {
+        best = beam_key(m, unsigned(at - mis));
+        break;
+      }
+    }
+    if (m != -INFINITY) break;  // (only fillers at the row's ends can be passed over)
+  }
+  // the bound: both threads of a pair count against half the pairs
+  unsigned long long pair = __shfl_xor_sync(0xffffffffu, best, 1);
+  pair = pair > best ? pair : best;
+  s_thin.best[tid] = pair;
+  __syncthreads();
+  {
+    int above = 0;
+#pragma unroll 8
+    for (int i = 0; i < kBeamGroups / 2; ++i)
+      above += s_thin.best[((tid & 1) * (kBeamGroups / 2) + i) * 2] > pair;
+    above += __shfl_xor_sync(0xffffffffu, above, 1);
+    if (above == p.k - 1 && pair != 0 && (tid & 1) == 0) s_thin.tau = pair;
+  }
+  __syncthreads();
+  unsigned long long tau = s_thin.tau;
+  // lists the thread's logits of the step at w, of the loads in `of`, whose keys reach
+  // tau; true when there are more than `most` in the list
+  auto list_step = [&](int w, uint32_t of, int most) -> bool {
+    bool over = false;
+    load(w, raw);
+    const float bound = tau == 0 ? -INFINITY : beam_value(unsigned(tau >> 32));
+    if (clean() >= bound)
+      for (uint32_t bits = at_or_above(bound) & of; bits; bits &= bits - 1) {
+        const int at = place(w, __ffs(bits) - 1);
+        if (at < mis || at >= w1) continue;
+        // (few: read again, rather than picked out of the registers)
+        const unsigned long long key = beam_key(beam_one(x0[at]), unsigned(at - mis));
+        if (key < tau) continue;
+        const int i = atomicAdd(&s_n, 1);
+        if (i < room) beam_cand[i] = key;
+        over = over || i >= most;
+      }
+    return over;
+  };
+  const bool look = best >= tau && best != 0;
+  if (look) {
+    const float bound = tau == 0 ? -INFINITY : beam_value(unsigned(tau >> 32));
+    for (int w = w0, i = 0; w < w1; w += TILE, ++i)
+      if (i >= kBeamSteps || step_max[i * kBeamThreads] >= bound) list_step(w, 0xffffffffu, room);
+  }
+  __syncthreads();
+  int n = s_n;
+  __syncthreads();
+  if (n > room) {
+    if (tid == 0) s_n = 0;
+    __syncthreads();
+    for (int w = w0; w < w1; w += TILE)
+      for (int j = 0; j < kBeamLoads; ++j) {
+        const uint32_t of = (VEC == 8 ? 0xffu : 0xfu) << (j * VEC);
+        const bool over = look && list_step(w, of, 2 * p.k + 32);
+        // (the answer has to be the block's: s_n may have moved on for some)
+        if (__syncthreads_or(over)) {
+          n = beam_thin(beam_cand, few, s_thin, s_n, p.k);
+          if (n == p.k) tau = beam_cand[n - 1] + 1;  // only better ones from now on
+          if (tid == 0) s_n = n;
+          __syncthreads();
+        }
+      }
+    n = s_n;
+    __syncthreads();
+  }
+  n = beam_thin(beam_cand, few, s_thin, n, p.k);
   const size_t at = size_t(blockIdx.x) * p.k;
-  const int kept = w0 < w1 ? min(s_n, p.k) : 0;
-  for (int i = tid; i < p.k; i += kBeamThreads) p.keys[at + i] = i < kept ? beam_cand[i] : 0ull;
+  for (int i = tid; i < p.k; i += kBeamThreads) p.keys[at + i] = i < n ? beam_cand[i] : 0ull;
   // the segment's maximum and sum
   float bm = m;
 #pragma unroll
@@ -331,7 +362,7 @@ __global__ void __launch_bounds__(kBeamThreads, 3) beam_segment_kernel(const Bea
   bm = s_max[0];
 #pragma unroll
   for (int w = 1; w < kBeamThreads / 32; ++w) bm = fmaxf(bm, s_max[w]);
-  sum = m == -INFINITY ? 0.0 : sum * double(expf(m - bm));
+  sum = m == -INFINITY ? 0.0 : sum * exp(double(m) - double(bm));
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   if (lane == 0) s_sum[warp] = sum;
@@ -348,7 +379,7 @@ __global__ void __launch_bounds__(kBeamThreads, 3) beam_segment_kernel(const Bea
 // lists. Lists are sorted, so the k best lie in the k lists with the best
 // heads: at most k*k candidates.
 __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const BeamSelectParams p) {
-  extern __shared__ unsigned long long beam_smem[];
+  extern __shared__ unsigned long long beam_lists[];
   __shared__ double s_off[kBeamMax];
   __shared__ float s_top[kBeamMax];
   __shared__ int s_n;
@@ -356,7 +387,7 @@ __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const Bea
   __shared__ unsigned s_tau_i;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int lists = p.beams * p.segments;
-  unsigned long long* head_v = beam_smem;                   // [lists] order of the head's score
+  unsigned long long* head_v = beam_lists;                  // [lists] order of the head's score
   unsigned* head_i = reinterpret_cast<unsigned*>(head_v + lists);  // [lists] its beam*vocab + token
   unsigned long long* cand_v = head_v + lists + (lists + 1) / 2;
   unsigned* cand_i = reinterpret_cast<unsigned*>(cand_v + p.k * p.k);

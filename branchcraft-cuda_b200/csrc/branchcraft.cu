@@ -1177,19 +1177,19 @@ cudaError_t launch_chunk(ChunkParams& p, const CUtensorMap* maps, const ChunkPla
 }
 
 // Rows are cut into the number of segments that takes the least time by count:
-// waves of three blocks a SM times a segment's steps and its fixed work (the first
-// bound and the last ranking, some three steps' time).
+// waves of four blocks a SM times a segment's steps and its fixed work (the bound,
+// the second look and the ranking, some six steps' time).
 struct BeamPlan {
   int segments, segment;
   BeamPlan(int rows, int vocab, int type_bytes, int dev) {
     const int tile = beam_tile(type_bytes);
     const int steps = (vocab + 15 + tile - 1) / tile;  // (from a 16-byte boundary on)
-    const long long slots = 3ll * (dev < 0 ? 148 : sm_count(dev));
+    const long long slots = 4ll * (dev < 0 ? 148 : sm_count(dev));
     long long least = -1;
     int per = steps;
     for (int s = 1; s <= steps && (s == 1 || (long long)rows * s <= 4 * slots); ++s) {
       const int each = (steps + s - 1) / s;
-      const long long time = (((long long)rows * s + slots - 1) / slots) * (each + 3);
+      const long long time = (((long long)rows * s + slots - 1) / slots) * (each + 6);
       if (least < 0 || time < least) {
         least = time;
         per = each;
@@ -1203,13 +1203,10 @@ struct BeamPlan {
 template <typename T>
 cudaError_t launch_beam_segments(const BeamSelectParams& p, int dev, cudaStream_t stream) {
   static std::atomic<uint64_t> configured{0};
-  const auto smem = [](int k) {
-    return size_t(beam_room(sizeof(T), k) + beam_few(sizeof(T), k)) * 8;
-  };
-  const cudaError_t e = raise_smem(beam_segment_kernel<T>, smem(kBeamMaxK), configured, dev);
+  const cudaError_t e = raise_smem(beam_segment_kernel<T>, beam_smem(kBeamMaxK), configured, dev);
   if (e != cudaSuccess) return e;
   return launch_dependent(beam_segment_kernel<T>, dim3(unsigned(p.batch) * p.beams * p.segments),
-                          kBeamThreads, smem(p.k), stream, p);
+                          kBeamThreads, beam_smem(p.k), stream, p);
 }
 
 int beam_type_bytes(int dtype) {
@@ -1428,8 +1425,8 @@ int bc_beam_select(int batch, int beams, int vocab, int k, int dtype, const void
                                      : launch_beam_segments<float>(p, dev, st);
   if (e != cudaSuccess) return e;
   static std::atomic<uint64_t> configured{0};
-  // (a request's lists: at most twelve blocks a SM, or one a beam)
-  e = raise_smem(beam_merge_kernel, beam_merge_smem(std::max(12 * sm_count(dev), kBeamMax), kBeamMaxK),
+  // (a request's lists: at most sixteen blocks a SM, or one a beam)
+  e = raise_smem(beam_merge_kernel, beam_merge_smem(std::max(16 * sm_count(dev), kBeamMax), kBeamMaxK),
                  configured, dev);
   if (e != cudaSuccess) return e;
   return launch_dependent(beam_merge_kernel, dim3(unsigned(batch)), kBeamMergeThreads,

@@ -64,6 +64,18 @@ def test_select_ties_and_order(bc, dtype):
     assert bc.beam_select(zeros, scores[:, :1].contiguous(), 5)[1].tolist() == [[0, 1, 2, 3, 4]]
 
 
+@pytest.mark.parametrize("dtype,vec", [(torch.float32, 4), (torch.float16, 8), (torch.bfloat16, 8)])
+@pytest.mark.parametrize("k", [64, 33])
+def test_select_best_in_few_threads(bc, dtype, vec, k):
+    """The best logits in the places of k - 1 pairs of threads (16-byte loads go to 256
+    threads in turn), more than a block lists at once: the second look is thinned."""
+    rows, vocab = 600, 40000
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randn(rows, 1, vocab, generator=g, device="cuda")
+    x[..., (torch.arange(vocab, device="cuda") // vec) % 256 < 2 * (k - 1)] += 40
+    check_select(bc, x.to(dtype), -torch.rand(rows, 1, generator=g, device="cuda"), k)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_select_infinities_and_nan(bc, dtype):
     g = torch.Generator(device="cuda").manual_seed(3)
