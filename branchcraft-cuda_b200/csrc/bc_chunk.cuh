@@ -45,7 +45,7 @@ constexpr int kChMergeThreads = 256;
 constexpr int kChTile = 128;      // keys of a tile: eight pages
 constexpr int kChDescs = 4;       // item descriptors in flight
 constexpr int kChMaxBatch = 4096;
-constexpr int kChMinPiece = 4;    // key tiles: the granularity of cuts inside an item
+constexpr int kChWhole = 5;       // key tiles of an item that is never split
 // What the shares balance, in the time of an ALT key tile: a DUAL tile is two, and
 // an item costs this much beside its tiles (its Q, its first scores, its epilogue).
 constexpr int kChItemCost = 5;
@@ -434,9 +434,9 @@ __global__ void __launch_bounds__(kChThreads, 1)
       // ------------------------------------------- scheduler and V producer
       // This block's share: from its own cut (found by lanes 0-15) up to the next
       // block's (lanes 16-31). Cuts inside an item fall on multiples of `grain`
-      // tiles from its start (a thirty-second of a share; at least kChMinPiece, half
-      // that in large shares: a piece costs its partial state's way through memory)
-      // or on its ends.
+      // tiles from its start (a thirty-second of a share, at least 2: eighths of a
+      // share left blocks a quarter apart, single tiles cost the prompts 2 %) or on
+      // its ends; an item of no more than kChWhole tiles has no cut.
       const int half = lane >> 4, hl = lane & 15;
       const int per_lane = (p.batch + 15) / 16;
       const int sb0 = min(p.batch, hl * per_lane), sb1 = min(p.batch, sb0 + per_lane);
@@ -487,15 +487,12 @@ __global__ void __launch_bounds__(kChThreads, 1)
       rem -= __shfl_sync(0xffffffffu, at, src, 16) * p.hkv;
       // its head and tile
       const int weight = chunk_weight(p, r.n - blk * block_tokens);
-      const long long share = cost / (gridDim.x * weight);  // in this item's tiles
-      const int grain = max(share >= 4 * kChMinPiece ? kChMinPiece / 2 : kChMinPiece,
-                            int(min(share / 32, 1ll << 20)));
+      const int grain = max(2, int(min(cost / gridDim.x / (32 * weight), 1ll << 20)));
       if (in) {
         head = int(double(rem) / double(n));
         off = max(int(rem - (long long)head * n) - kChItemCost, 0) / weight;
         n = (n - kChItemCost) / weight;
-        // (an item of no more than a piece and a tile stays whole)
-        off = n <= kChMinPiece + 1 ? (2 * off > n ? n : 0) : (off + grain / 2) / grain * grain;
+        off = n <= kChWhole ? (2 * off > n ? n : 0) : (off + grain / 2) / grain * grain;
         if (off > 0 && n - off < (grain + 1) / 2) {  // the next item's start
           off = 0;
           if (++head == p.hkv) {
@@ -835,34 +832,47 @@ __global__ void __launch_bounds__(kChThreads, 1)
         // scale (> 0) waits for the exponent's multiply-add.
         if constexpr (MOD & 1) {
           // cap * tanh(u), u = x scale / cap. While the warp's |u| stay below 3/4, as
-          // scores of a model trained with its cap do, by the polynomial
-          // v + v t P(t), v = x scale log2(e), t = u^2, P of degree 4 with the least
-          // largest error of tanh on [0, 3/4] (1.3e-8, fitted for this kernel): two
-          // scores an instruction. Else cap - 2 cap / (1 + exp(2 u)), two more
-          // results of the exponential unit a score, which bounds the softmax.
+          // scores of a model trained with its cap do, as x Q(x^2), an odd polynomial
+          // of u of degree 11 with the least largest error of tanh on [0, 3/4] (1.3e-8,
+          // fitted for this kernel; of degree 7 below 0.35: 8.8e-9), cap and scale in
+          // its coefficients: 7 (5) multiply-adds a score. Else cap - 2 cap / (1 +
+          // exp(2 u)), two more results of the exponential unit, which bounds the
+          // softmax. (Multiplying out u, u^2 and v apart took 10, and the FMA pipe
+          // 2300 cycles a tile and warp against 1400 for the rest.)
           float big = 0.f;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int e = 0; e < 32; e += 2)
               big = fmax3_abs(big, __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-          if (__all_sync(0xffffffffu, big * p.cap_u < 0.75f)) {
-            const uint64_t arg = pair_of(p.cap_u, p.cap_u), sl = pair_of(p.scale_log2, p.scale_log2);
-            const uint64_t c1 = pair_of(-0.33332908153533936f, -0.33332908153533936f),
-                           c2 = pair_of(0.13324248790740967f, 0.13324248790740967f),
-                           c3 = pair_of(-0.05328230932354927f, -0.05328230932354927f),
-                           c4 = pair_of(0.01945533975958824f, 0.01945533975958824f),
-                           c5 = pair_of(-0.004626113455742598f, -0.004626113455742598f);
+          const float most = big * p.cap_u;
+          const float u2 = p.cap_u * p.cap_u;
+          auto both = [](float x) { return pair_of(x, x); };
+          auto odd = [&](auto terms, float c1, float c2, float c3, float c4, float c5) {
+            const uint64_t k0 = both(p.scale_log2), k1 = both(c1 * u2 * p.scale_log2),
+                           k2 = both(c2 * u2 * u2 * p.scale_log2),
+                           k3 = both(c3 * u2 * u2 * u2 * p.scale_log2),
+                           k4 = both(c4 * u2 * u2 * (u2 * u2) * p.scale_log2),
+                           k5 = both(c5 * u2 * u2 * (u2 * u2) * u2 * p.scale_log2);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
               for (int e = 0; e < 32; e += 2) {
                 const uint64_t x = pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-                const uint64_t u = mul2(x, arg), t = mul2(u, u), v = mul2(x, sl);
-                const uint64_t P = fma2(t, fma2(t, fma2(t, fma2(t, c5, c4), c3), c2), c1);
-                const uint64_t y = fma2(v, mul2(t, P), v);
+                const uint64_t t = mul2(x, x);
+                uint64_t q = k3;
+                if constexpr (decltype(terms)::value == 5) q = fma2(t, fma2(t, k5, k4), k3);
+                q = fma2(t, fma2(t, fma2(t, q, k2), k1), k0);
+                const uint64_t y = mul2(x, q);
                 asm("mov.b64 {%0, %1}, %2;" : "=r"(s[c][e]), "=r"(s[c][e + 1]) : "l"(y));
               }
+          };
+          if (__all_sync(0xffffffffu, most < 0.35f)) {
+            odd(std::integral_constant<int, 3>{}, -0.3333243131637573f, 0.13294382393360138f,
+                -0.04885116592049599f, 0.f, 0.f);
+          } else if (__all_sync(0xffffffffu, most < 0.75f)) {
+            odd(std::integral_constant<int, 5>{}, -0.33332908153533936f, 0.13324248790740967f,
+                -0.05328230932354927f, 0.01945533975958824f, -0.004626113455742598f);
           } else {
             const float arg = 2.f * 1.4426950408889634f * p.cap_u;
 #pragma unroll

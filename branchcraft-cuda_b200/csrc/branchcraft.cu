@@ -1131,8 +1131,7 @@ struct ChunkPlan {
     const long long items = ((long long)tokens / (2 * tile) + std::min(s->batch, tokens)) * s->kv_heads;
     blocks = int(std::min<long long>(std::min(dev < 0 ? 148 : sm_count(dev), 160), items * key_tiles));
     rows = tokens <= tile ? (tokens * group + 31) / 32 * 32 : 256;
-    // (an item of kChMinPiece + 1 tiles is never split)
-    bytes = key_tiles <= kChMinPiece + 1
+    bytes = key_tiles <= kChWhole
                 ? 0
                 : size_t(blocks) * (2 * size_t(rows) * (s->dim * 4 + 8) + 32);
   }
