@@ -434,8 +434,9 @@ __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const Bea
   };
   for (int l = tid; l < lists; l += kBeamMergeThreads) {
     const unsigned long long key = keys[size_t(l) * p.k];
-    head_v[l] = value(l, key);
-    head_i[l] = index(l, key);
+    // (a segment past a row's end has an empty list: behind all others)
+    head_v[l] = key == 0 ? 0ull : value(l, key);
+    head_i[l] = key == 0 ? 0xffffffffu - unsigned(l) : index(l, key);
   }
   __syncthreads();
   for (int l = tid; l < lists; l += kBeamMergeThreads) {  // the k-th best head

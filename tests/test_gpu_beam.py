@@ -76,6 +76,20 @@ def test_select_best_in_few_threads(bc, dtype, vec, k):
     check_select(bc, x.to(dtype), -torch.rand(rows, 1, generator=g, device="cuda"), k)
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 4096), (torch.float32, 8192),
+                                         (torch.bfloat16, 8192), (torch.float16, 16384)])
+def test_select_whole_steps(bc, dtype, vocab):
+    """Rows of exactly a block's step, whose last segment may be empty: the best k are
+    one of each beam."""
+    beams = 16
+    x = torch.randn(2, beams, vocab, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    for w in range(beams):
+        x[:, w, 100 * w + 3] = 30.0 + w / 4
+    scores = torch.linspace(-3, 0, beams, device="cuda").repeat(2, 1).contiguous()
+    got = check_select(bc, x.to(dtype), scores, beams)
+    assert sorted(got[2][0].tolist()) == list(range(beams))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_select_infinities_and_nan(bc, dtype):
     g = torch.Generator(device="cuda").manual_seed(3)
