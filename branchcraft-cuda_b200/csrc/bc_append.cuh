@@ -318,6 +318,7 @@ struct AppendKvParams {
 };
 
 constexpr int kAppendThreads = 256;
+constexpr int kAppendVecs = 4;
 
 // Blocks [0, token_blocks) copy rows, K (blockIdx.y 0) or V (1); block
 // token_blocks + c copies clone c's valid slots. A clone reads slots below its
@@ -350,16 +351,30 @@ __global__ void __launch_bounds__(kAppendThreads)
   const long long xs = is_v ? p.v_stride : p.k_stride;
   const int t0 = int(blockIdx.x) * tokens_per_block;
   const int nt = min(tokens_per_block, p.tokens - t0);
-  for (int i = threadIdx.x; i < nt * p.row_vecs; i += kAppendThreads) {
-    const int t = t0 + i / p.row_vecs, r = i % p.row_vecs;
-    const int slot = p.slot_map[t];
-    if (slot < 0 || slot >= p.physical_pages * kPageSize) {
-      if (slot != -1 && r == 0) atomicOr(p.err, kErrCommitIndex);
-      continue;
+  // kAppendVecs pieces of a thread in flight before the first is stored (the
+  // stores could be the next loads' sources for all the compiler knows): 18k rows of
+  // 2 KB went from 5.5 to 6 TB/s.
+  for (int i0 = threadIdx.x; i0 < nt * p.row_vecs; i0 += kAppendVecs * kAppendThreads) {
+    uint4 val[kAppendVecs];
+    long long to[kAppendVecs];
+#pragma unroll
+    for (int j = 0; j < kAppendVecs; ++j) {
+      const int i = i0 + j * kAppendThreads;
+      to[j] = -1;
+      if (i >= nt * p.row_vecs) continue;
+      const int t = t0 + i / p.row_vecs, r = i % p.row_vecs;
+      const int slot = p.slot_map[t];
+      if (slot < 0 || slot >= p.physical_pages * kPageSize) {
+        if (slot != -1 && r == 0) atomicOr(p.err, kErrCommitIndex);
+        continue;
+      }
+      val[j] = __ldcs(x + t * xs + r);
+      to[j] = (slot / kPageSize) * p.block_stride + (slot % kPageSize) * p.slot_stride +
+              (r / p.head_vecs) * p.head_stride + r % p.head_vecs;
     }
-    const uint4 val = x[t * xs + r];
-    cache[(slot / kPageSize) * p.block_stride + (slot % kPageSize) * p.slot_stride +
-          (r / p.head_vecs) * p.head_stride + r % p.head_vecs] = val;
+#pragma unroll
+    for (int j = 0; j < kAppendVecs; ++j)
+      if (to[j] >= 0) cache[to[j]] = val[j];
   }
 }
 

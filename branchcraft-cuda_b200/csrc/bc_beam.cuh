@@ -527,9 +527,9 @@ __global__ void __launch_bounds__(kReorderWarps * 32) beam_rows_kernel(const Bea
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   grid_launch_dependents();
   grid_dependency_wait();
-  const long long item = (long long)blockIdx.x * kReorderWarps + warp;
-  if (item >= (long long)p.batch * p.words) return;
-  const int b = int(item / p.words), word = int(item % p.words), c = word * 32 + lane;
+  const unsigned item = blockIdx.x * kReorderWarps + warp;  // (words of all marks: below 2^26)
+  if (item >= unsigned(p.batch) * p.words) return;
+  const int b = int(item / unsigned(p.words)), word = int(item % unsigned(p.words)), c = word * 32 + lane;
   int* child = s_child[warp];
   int* parent = s_parent[warp];
   int (*page)[32] = s_pages[warp];
@@ -609,11 +609,12 @@ __global__ void __launch_bounds__(kReleaseThreads) beam_release_kernel(const Bea
   if (tid == 0) s_over = 0;
   grid_dependency_wait();
   __syncthreads();
-  const long long total = (long long)p.batch * p.beams_in * p.words;
-  const long long per = (total + kWarps - 1) / kWarps;
-  const long long w0 = min(total, warp * per), w1 = min(total, w0 + per);
-  auto page_at = [&](long long w, int bit) -> int {
-    return p.pages_in[size_t(w / p.words) * p.max_pages + size_t(w % p.words) * 32 + bit];
+  const int total = p.batch * p.beams_in * p.words;  // (below 2^26)
+  const int per = (total + kWarps - 1) / kWarps;
+  const int w0 = min(total, warp * per), w1 = min(total, w0 + per);
+  auto page_at = [&](int w, int bit) -> int {
+    const unsigned row = unsigned(w) / unsigned(p.words);
+    return p.pages_in[size_t(row) * p.max_pages + (unsigned(w) - row * p.words) * 32 + bit];
   };
   auto count_of = [&](int page) { return *reinterpret_cast<volatile int*>(&p.refcount[page]); };
   const int count = *p.free_count_in;
@@ -621,14 +622,16 @@ __global__ void __launch_bounds__(kReleaseThreads) beam_release_kernel(const Bea
   // the marked pages that became free: their marks stay, and they are listed
   int2* list = release_list + warp * kReleaseList;  // (place, page)
   int n = 0;
-  for (long long g = w0; g < w1; g += 32) {
-    const unsigned word = g + lane < w1 ? p.marks[g + lane] : 0u;
+  unsigned ahead = w0 + lane < w1 ? p.marks[w0 + lane] : 0u;
+  for (int g = w0; g < w1; g += 32) {
+    const unsigned word = ahead;
+    ahead = g + 32 + lane < w1 ? p.marks[g + 32 + lane] : 0u;
     unsigned some = __ballot_sync(0xffffffffu, word != 0u);
-    while (some) {  // four words of marks at a time, a lane a bit
-      int src[4], page[4], rc[4];
-      unsigned bits[4];
+    while (some) {  // eight words of marks at a time, a lane a bit
+      int src[8], page[8], rc[8];
+      unsigned bits[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         src[i] = some ? __ffs(some) - 1 : -1;
         bits[i] = __shfl_sync(0xffffffffu, word, max(src[i], 0));
         if (src[i] < 0) bits[i] = 0u;
@@ -636,12 +639,12 @@ __global__ void __launch_bounds__(kReleaseThreads) beam_release_kernel(const Bea
         page[i] = (bits[i] >> lane) & 1u ? page_at(g + src[i], lane) : -1;
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) rc[i] = page[i] >= 0 ? count_of(page[i]) : 1;
+      for (int i = 0; i < 8; ++i) rc[i] = page[i] >= 0 ? count_of(page[i]) : 1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const unsigned left = __ballot_sync(0xffffffffu, rc[i] == 0);
         const int at = n + __popc(left & ((1u << lane) - 1));
-        if (rc[i] == 0 && at < kReleaseList) list[at] = make_int2(int((g + src[i]) * 32 + lane), page[i]);
+        if (rc[i] == 0 && at < kReleaseList) list[at] = make_int2((g + src[i]) * 32 + lane, page[i]);
         n += __popc(left);
         if (lane == 0 && src[i] >= 0 && left != bits[i]) p.marks[g + src[i]] = left;
       }
@@ -650,51 +653,76 @@ __global__ void __launch_bounds__(kReleaseThreads) beam_release_kernel(const Bea
   if (n > kReleaseList && lane == 0) s_over = 1;
   __syncthreads();
   const bool listed = s_over == 0;
-  // what is left, in order: (place, page) of this lane's next entry, or none
-  auto each = [&](auto&& f) {
-    if (listed) {
-      for (int i0 = 0; i0 < n; i0 += 32) {
-        const bool in = i0 + lane < n;
-        const int2 e = in ? list[i0 + lane] : make_int2(0, 0);
-        f(in, e.x, e.y);
-      }
-    } else {
-      for (long long w = w0; w < w1; ++w) {
+  auto push = [&](long long at, int page) {
+    if (at >= 0 && at < p.physical_pages)
+      p.free_stack[at] = page;
+    else
+      atomicOr(p.err, kErrPageRange);
+    p.refcount[page] = 0;
+  };
+  int freed = 0;
+  // the pushes of the warps before this one
+  auto before_of = [&](int mine) -> int {
+    if (lane == 0) s_warp[warp] = mine;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += s_warp[w];
+      freed += s_warp[w];
+    }
+    return before;
+  };
+  if (listed) {  // (a lane's entries in registers: the phases' accesses overlap)
+    constexpr int kMine = kReleaseList / 32;
+    int2 e[kMine];
+    unsigned wins[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const bool in = i * 32 + lane < n;
+      e[i] = in ? list[i * 32 + lane] : make_int2(-1, -1);
+      if (in) atomicMin(&p.refcount[e[i].y], -e[i].x - 1);
+    }
+    __syncthreads();
+    int now[kMine], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) now[i] = e[i].x >= 0 ? count_of(e[i].y) : 0;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      wins[i] = __ballot_sync(0xffffffffu, e[i].x >= 0 && now[i] == -e[i].x - 1);
+      mine += __popc(wins[i]);
+    }
+    long long at = (long long)count + before_of(mine);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      if ((wins[i] >> lane) & 1u) push(at + __popc(wins[i] & ((1u << lane) - 1)), e[i].y);
+      at += __popc(wins[i]);
+    }
+  } else {
+    // (this lane's bit of each of the warp's words, in order)
+    auto each = [&](auto&& f) {
+      for (int w = w0; w < w1; ++w) {
         const unsigned bits = p.marks[w];
         if (bits == 0u) continue;
         const bool in = (bits >> lane) & 1u;
-        f(in, int(w * 32 + lane), in ? page_at(w, lane) : 0);
+        f(in, w * 32 + lane, in ? page_at(w, lane) : 0);
       }
-    }
-  };
-  each([&](bool in, int place, int page) {
-    if (in) atomicMin(&p.refcount[page], -place - 1);
-  });
-  __syncthreads();
-  int mine = 0;
-  each([&](bool in, int place, int page) {
-    mine += __popc(__ballot_sync(0xffffffffu, in && count_of(page) == -place - 1));
-  });
-  if (lane == 0) s_warp[warp] = mine;
-  __syncthreads();
-  int before = 0, freed = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s_warp[w];
-    freed += s_warp[w];
+    };
+    each([&](bool in, int place, int page) {
+      if (in) atomicMin(&p.refcount[page], -place - 1);
+    });
+    __syncthreads();
+    int mine = 0;
+    each([&](bool in, int place, int page) {
+      mine += __popc(__ballot_sync(0xffffffffu, in && count_of(page) == -place - 1));
+    });
+    long long at = (long long)count + before_of(mine);
+    each([&](bool in, int place, int page) {
+      const bool won = in && count_of(page) == -place - 1;
+      const unsigned wins = __ballot_sync(0xffffffffu, won);
+      if (won) push(at + __popc(wins & ((1u << lane) - 1)), page);
+      at += __popc(wins);
+    });
   }
-  each([&](bool in, int place, int page) {
-    const bool won = in && count_of(page) == -place - 1;
-    const unsigned wins = __ballot_sync(0xffffffffu, won);
-    if (won) {
-      const long long at = (long long)count + before + __popc(wins & ((1u << lane) - 1));
-      if (at >= 0 && at < p.physical_pages)
-        p.free_stack[at] = page;
-      else
-        atomicOr(p.err, kErrPageRange);
-      p.refcount[page] = 0;
-    }
-    before += __popc(wins);
-  });
   if (tid == 0) *p.free_count = int(min((long long)count + freed, (long long)p.physical_pages));
 }
 

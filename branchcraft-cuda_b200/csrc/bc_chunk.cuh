@@ -487,11 +487,13 @@ __global__ void __launch_bounds__(kChThreads, 1)
       rem -= __shfl_sync(0xffffffffu, at, src, 16) * p.hkv;
       // its head and tile
       const int weight = chunk_weight(p, r.n - blk * block_tokens);
-      const int grain = max(2, int(min(cost / gridDim.x / (32 * weight), 1ll << 20)));
+      const int grain = max(2, int(fminf(float(cost) / float(gridDim.x * 32 * weight), 1048576.f)));
       if (in) {
-        head = int(double(rem) / double(n));
-        off = max(int(rem - (long long)head * n) - kChItemCost, 0) / weight;
-        n = (n - kChItemCost) / weight;
+        head = int(float(rem) / float(n));  // (rem < n * hkv; put right below)
+        while ((long long)head * n > rem) --head;
+        while ((long long)(head + 1) * n <= rem) ++head;
+        off = max(int(rem - (long long)head * n) - kChItemCost, 0) >> (weight - 1);
+        n = (n - kChItemCost) >> (weight - 1);
         off = n <= kChWhole ? (2 * off > n ? n : 0) : (off + grain / 2) / grain * grain;
         if (off > 0 && n - off < (grain + 1) / 2) {  // the next item's start
           off = 0;

@@ -1303,7 +1303,7 @@ int bc_append_kv(const bc_shape* s, int tokens, const void* k, long long k_strid
   p.clones = clones;
   p.counts = counts;
   p.err = err;
-  const int per_block = std::max(1, 4 * kAppendThreads / p.row_vecs);
+  const int per_block = std::max(1, kAppendVecs * kAppendThreads / p.row_vecs);
   const int token_blocks = (tokens + per_block - 1) / per_block;
   return launch_dependent(append_kv_kernel, dim3(unsigned(token_blocks + max_clones), 2),
                           kAppendThreads, 0, static_cast<cudaStream_t>(stream), p, token_blocks,
