@@ -203,8 +203,8 @@ def chunk_attention(q, k, v, pages, query_start, lengths, scale=None, softcap=0.
     `window` keeps the last keys, `key_start` [tokens] is a token's first key (packed documents);
     `softcap` caps scores by a tanh, `alibi_slopes` [Hq] take slope * distance off. Output of q's
     type; rows of tokens in no request are unspecified (chunk_attention_out leaves them)."""
-    return _chunk_attention(q, k, v, pages, query_start, lengths, scale,
-                                                 softcap, window, alibi_slopes, prefix, key_start)
+    return _chunk_attention(q, k, v, pages, query_start, lengths, scale, softcap, window,
+                            alibi_slopes, prefix, key_start)
 
 
 def chunk_attention_out(q, k, v, pages, query_start, lengths, output, scale=None, softcap=0.0,
@@ -226,11 +226,9 @@ def beam_reorder(pages, lengths, parents, refcount, free_stack, free_count):
     """Page tables [B, beams, max_pages] after parents [B, new beams] (-1 drops a row): returns
     (pages, lengths, refcount, free_stack, free_count), every new row forked from its parent,
     every old one released, unheld pages pushed on the free stack."""
-    return _beam_reorder(pages, lengths, parents, refcount, free_stack,
-                                              free_count)
+    return _beam_reorder(pages, lengths, parents, refcount, free_stack, free_count)
 
 
 def beam_reorder_(pages, lengths, parents, refcount, free_stack, free_count):
     """beam_reorder updating the pool's state in place; returns (pages, lengths)."""
-    return _beam_reorder_(pages, lengths, parents, refcount, free_stack,
-                                               free_count)
+    return _beam_reorder_(pages, lengths, parents, refcount, free_stack, free_count)

@@ -381,3 +381,18 @@ def test_refusals(bc):
     empty = bc.chunk_attention(f["q"][:0], f["k"], f["v"], f["pages"], f["query_start"] * 0,
                                f["lengths"])
     assert empty.shape == (0, 8, 64)
+
+
+@pytest.mark.parametrize("dtype,dim", [(F16, 64), (BF16, 128)])
+def test_key_starts_in_any_order(bc, dtype, dim):
+    f = make([300, 1, 77], [520, 400, 77], 4, 2, dim, dtype, seed=11)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    start = torch.randint(-5, 560, (378,), generator=g, device="cuda", dtype=torch.int32)
+    check(bc, f, key_start=start)
+    check(bc, f, key_start=start, window=40)
+
+
+def test_as_many_requests_as_allowed(bc):
+    new = [(b * 7) % 3 for b in range(4096)]
+    lens = [n + (b * 5) % 40 for b, n in enumerate(new)]
+    check(bc, make(new, lens, 2, 1, 64, F16, seed=12))

@@ -167,3 +167,17 @@ def test_cpu_tensors_are_rejected():
                  lambda: B.beam_reorder(i[None, None], i[None], i[None], i, i, i)):
         with pytest.raises((RuntimeError, NotImplementedError)):
             call()
+
+
+def test_chunk_limits_and_output_alignment():
+    def call(s, output):
+        layout = C.KvLayout(2048, 128, 64)
+        opt = C.ChunkOptions(0.125, 0.0, 0, None, None, None)
+        size = C.chunk_workspace_bytes(s, 3)
+        return LIB.bc_chunk_attention(ctypes.byref(s), 3, 0, P, 512, P, P, ctypes.byref(layout), P,
+                                      P, P, ctypes.byref(opt), output, 0, P, size, None)
+
+    assert call(shape(batch=4097), P) == 1
+    assert C.chunk_workspace_bytes(shape(batch=4097), 3) == 0
+    assert call(shape(), ctypes.c_void_p(4096 + 16)) == 1
+    assert call(shape(), ctypes.c_void_p(4096 + 2)) == 1
