@@ -45,6 +45,16 @@ class PagedSequences:
         (query_start [rows + 1], positions [tokens]): which of the tokens are a row's, and
         where they stand in it (-1: in no row). When the plan fails (see check) nothing is
         appended and no token is in any row."""
+        # (refused here: the plan below changes the tables before the rows are looked at)
+        heads, dim = self.k.shape[2:]
+        for t in (k, v):
+            if (t.dim() != 3 or t.shape[0] != k.shape[0] or tuple(t.shape[1:]) != (heads, dim)
+                    or t.dtype != self.k.dtype or t.device != self.k.device
+                    or t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim)
+                    or (t.shape[0] > 1 and (t.stride(0) < 0 or t.stride(0) % 8))
+                    or t.data_ptr() % 16):
+                raise ValueError("k and v must be [tokens, KV heads, head dim] of the cache's type "
+                                 "and device, each token's heads contiguous, 16-byte aligned")
         query_start, slot_map, positions, clones, counts = append_plan_(
             self.pages, self.lengths, new_tokens, self.refcount, self.free_stack,
             self.free_count, k.shape[0])

@@ -181,3 +181,23 @@ def test_chunk_limits_and_output_alignment():
     assert C.chunk_workspace_bytes(shape(batch=4097), 3) == 0
     assert call(shape(), ctypes.c_void_p(4096 + 16)) == 1
     assert call(shape(), ctypes.c_void_p(4096 + 2)) == 1
+
+
+def test_append_refuses_rows_before_it_plans(monkeypatch):
+    from branchcraft_torch import sequences
+
+    def planned(*_):
+        raise AssertionError("planned before the rows were checked")
+
+    monkeypatch.setattr(sequences, "append_plan_", planned)
+    seq = sequences.PagedSequences(2, 1, 4, 8, 2, 64, device="cpu")
+    new = torch.ones(2, dtype=torch.int32)
+    good = torch.zeros(2, 2, 64, dtype=torch.float16)
+    wide = torch.zeros(2, 2, 68, dtype=torch.float16)
+    for bad in (good[:1], good[:, :1], good[..., :32], good.float(), good[0],
+                torch.zeros(2, 64, 2, dtype=torch.float16).transpose(1, 2), wide[..., :64],
+                torch.zeros(257, dtype=torch.float16)[1:].view(2, 2, 64)):
+        with pytest.raises(ValueError):
+            seq.append(good, bad, new)
+    with pytest.raises(AssertionError):
+        seq.append(good, good, new)
