@@ -59,7 +59,8 @@ class PagedSequences:
             self.pages, self.lengths, new_tokens, self.refcount, self.free_stack,
             self.free_count, k.shape[0])
         append_kv_(self.k, self.v, k, v, slot_map, clones, counts)
-        self.counts = counts
+        # (in place: a replayed step reports to the same tensor as the calls between)
+        self.counts.copy_(counts)
         return query_start, positions
 
     def attend(self, q: torch.Tensor, query_start: torch.Tensor, **options) -> torch.Tensor:

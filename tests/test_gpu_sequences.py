@@ -222,3 +222,27 @@ def test_schemas(bc):
     rows = ints([[[0, -1], [1, -1]]])
     t(op.beam_reorder.default, (rows, ints([[3, 5]]), ints([[1, 1]]), *state), test_utils=utils)
     t(op.beam_reorder_.default, (rows, ints([[3, 5]]), ints([[1, 1]]), *state), test_utils=utils)
+
+
+def test_check_follows_replays(bc):
+    from branchcraft_torch.sequences import PagedSequences
+
+    seq = PagedSequences(1, 1, 4, 2, 1, 64)
+    row = torch.zeros(16, 1, 64, dtype=torch.float16, device="cuda")
+    new = ints([16])
+    seq.append(row, row, ints([0]))  # (a first call outside the capture)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        seq.append(row, row, new)
+    seq.append(row, row, new)
+    seq.check()
+    graph.replay()
+    seq.check()
+    assert seq.lengths.tolist() == [32]
+    graph.replay()  # both pages are in use
+    with pytest.raises(RuntimeError, match="exhausted"):
+        seq.check()
+    assert seq.lengths.tolist() == [32]
+    seq.append(row, row, ints([0]))
+    seq.check()
