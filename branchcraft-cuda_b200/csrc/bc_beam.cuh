@@ -209,6 +209,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const Bea
   const int mis = int((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
   const T* x0 = x - mis;
   const int w0 = seg * p.segment, w1 = min(w0 + p.segment, p.vocab + mis);
+  const float score = p.scores[row];
   auto load = [&](int w, uint32_t (&raw)[16]) {
 #pragma unroll
     for (int j = 0; j < kBeamLoads; ++j) {
@@ -231,6 +232,20 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const Bea
   };
   uint32_t raw[16], next[16];
   if (w0 < w1) load(w0, raw);
+  // A beam that is out: all its pairs score -inf, so its first tokens are its best,
+  // whatever their logits. (Looked at with the first logits on their way: beside
+  // them, the score costs no wait of its own.)
+  if (beam_score(score) == -INFINITY) {
+    const int first = max(w0 - mis, 0);
+    for (int i = tid; i < p.k; i += kBeamThreads)
+      p.keys[size_t(blockIdx.x) * p.k + i] =
+          first + i < w1 - mis ? beam_key(-INFINITY, unsigned(first + i)) : 0ull;
+    if (tid == 0) {
+      p.seg_max[blockIdx.x] = -INFINITY;
+      p.seg_sum[blockIdx.x] = 0.0;
+    }
+    return;
+  }
   auto val = [&](int j) { return beam_float(raw[j / PW], j % PW, kType); };
   // the thread's logits at or above `bound`, a bit each
   auto at_or_above = [&](float bound) -> uint32_t {

@@ -261,3 +261,25 @@ def test_reorder_refusals(bc):
                  (pages, lengths, good, state[0], state[1][:3].contiguous(), state[2])):
         with pytest.raises((RuntimeError, NotImplementedError)):
             bc.beam_reorder(*args)
+
+
+@pytest.mark.parametrize("out", [-math.inf, math.nan])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_select_beams_that_are_out(bc, dtype, out):
+    """The pairs of a beam that is out score -inf like any other impossible pair: the
+    lowest index first among all of them, whatever its logits."""
+    up = torch.arange(5.0, device="cuda").to(dtype)[None, None]
+    got = check_select(bc, up, torch.full((1, 1), out, device="cuda"), 2)
+    assert got[1].tolist() == [[0, 1]]
+    g = torch.Generator(device="cuda").manual_seed(9)
+    for beams, vocab, k, allowed in ((2, 1000, 8, 3), (3, 17, 40, 5), (4, 40001, 64, 20),
+                                     (2, 200001, 64, 1), (1, 33000, 64, 0), (8, 300, 64, 50)):
+        for dead in ([0], list(range(beams)), list(range(1, beams)), [beams - 1]):
+            x = torch.randn(2, beams, vocab, generator=g, device="cuda").to(dtype)
+            x[..., torch.randperm(vocab, generator=g, device="cuda")[allowed:]] = -math.inf
+            x[:, dead] = torch.randn(2, len(dead), vocab, generator=g, device="cuda").to(dtype)
+            scores = -torch.rand(2, beams, generator=g, device="cuda")
+            scores[0, dead] = out
+            check_select(bc, x, scores, k)
+            scores[1, dead] = out
+            check_select(bc, x, scores, min(k, allowed + 1))
