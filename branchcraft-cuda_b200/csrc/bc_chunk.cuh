@@ -5,7 +5,8 @@
 //   hi = max(p + 1, prefix_b), lo = max(0, p + 1 - window, key_start_t),
 // with scores x_j = scale q.k_j, capped to softcap tanh(x_j / softcap), less
 // slope_h |p - j|; the output is sum_j exp(x_j - m) v_j / sum_j exp(x_j - m),
-// zeros where no key is seen.
+// zeros where no key is seen. Scores that are not finite go through this formula
+// as they are: a row that sees +inf or NaN, or nothing but -inf, is NaN.
 //
 // Work. A row tile is up to 128 (token, query head of one KV head) pairs, so a
 // K/V tile read once serves the whole group; an item is one block of two row
@@ -273,7 +274,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
                      const __grid_constant__ CUtensorMap vmap) {
   using G = ChunkGeom<D>;
   constexpr int KB = G::KB, NK = G::kKStages, NV = G::kVStages;
-  constexpr float kNegInf = -INFINITY;
+  constexpr float kNegInf = -INFINITY, kLowest = -3.402823466e38f;
   constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
   constexpr uint32_t kIdescS = umma_idesc_f16(128, kChTile, false, false) | kBf16;
   constexpr uint32_t kIdescPV = umma_idesc_f16(128, D, false, true) | kBf16;
@@ -1005,6 +1006,10 @@ __global__ void __launch_bounds__(kChThreads, 1)
       if (sc > 0) ok = __all_sync(0xffffffffu, mbar_wait(&p_done[grp], (sc - 1) & 1));
       if (!ok) break;
       tc_fence_after();
+      // A row that saw keys, but no score above -inf: a reference of its own tells it
+      // from one that saw none (its O is 0, its l 0, or NaN where a score was NaN).
+      if (m_ref == kNegInf && max(lo, d.t0 * kChTile) < min(hi, min(d.hi, (d.t0 + d.nt) * kChTile)))
+        m_ref = kLowest;
       // The row's factor on each group's O (0 where it saw no key), its columns
       // [c0, c1), and where they go.
       float f0, f1 = 0.f, m_out = m_ref, l_out = l_sum;
@@ -1029,7 +1034,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
         f0 = m_ref == kNegInf ? 0.f : 1.f;
       }
       if (d.slot < 0) {
-        const float inv = l_out > 0.f ? 1.f / l_out : 0.f;
+        const float inv = m_out == kNegInf ? 0.f : 1.f / l_out;  // (l of 0 or NaN: NaN below)
         f0 *= inv;
         f1 *= inv;
       }
@@ -1182,7 +1187,7 @@ __global__ void __launch_bounds__(kChMergeThreads) chunk_merge_kernel(const Chun
       }
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = m == -INFINITY ? 0.f : 1.f / l;
   const size_t at = (size_t(first + tok) * p.hq + head * p.group + (row % 128) % p.group) * D +
                     warp * N * 4;
 #pragma unroll

@@ -395,7 +395,8 @@ typedef struct bc_chunk_options {
  * elements between tokens) and the last ones of its lengths[b] keys; the token
  * at position p sees the keys j with lo <= j < hi, hi = max(p + 1, prefix[b])
  * (at most lengths[b]), lo = max(0, p + 1 - window, key_start[t]). A token
- * without a key gets zeros. One token per request is a decode step. dtype
+ * without a key gets zeros; one that sees a score of NaN or +inf, or none above
+ * -inf, gets NaN. One token per request is a decode step. dtype
  * (BC_F16 or BC_BF16) is that of q, k, v and, unless output_f32 != 0, of output
  * [tokens, query_heads, dim], contiguous; rows in no request are left as they
  * are. Sums are held in FP32; probabilities are rounded to dtype before the
