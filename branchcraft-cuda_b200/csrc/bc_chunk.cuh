@@ -72,7 +72,7 @@ struct ChunkParams {
   void* out;                  // [tokens, hq, D]
   int out_f32;
   float scale_log2;           // scale * log2(e)
-  float cap_log2, cap_u;      // softcap * log2(e), scale / softcap
+  float cap_log2, cap_u;      // softcap * log2(e), scale / softcap, both finite
   // workspace of split items (null when none can be split)
   float4* part_o;             // [blocks * 2][D / 4][part_rows]
   float2* part_ml;            // [blocks * 2][part_rows]
@@ -248,6 +248,18 @@ __device__ __forceinline__ void add_pair(float& a0, float& a1, float b0, float b
       "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
       : "+f"(a0), "+f"(a1)
       : "f"(b0), "f"(b1));
+}
+
+// tanh(u) / u in powers of u^2: up to |u| = 0.35, and up to 3/4.
+struct TanhLow {
+  float c[4] = {1.f, -0.3333243131637573f, 0.13294382393360138f, -0.04885116592049599f};
+};
+struct TanhMid {
+  float c[6] = {1.f, -0.33332908153533936f, 0.13324248790740967f, -0.05328230932354927f,
+                0.01945533975958824f, -0.004626113455742598f};
+};
+__device__ __forceinline__ float tanh_far(float u, float cap) {
+  return fmaf(-2.f * cap, fast_rcp(1.f + fast_exp2(u * (2.f * 1.4426950408889634f))), cap);
 }
 
 // Largest magnitude of three.
@@ -834,56 +846,54 @@ __global__ void __launch_bounds__(kChThreads, 1)
         // scale (> 0) waits for the exponent's multiply-add.
         if constexpr (MOD & 1) {
           // cap * tanh(u), u = x scale / cap. While the warp's |u| stay below 3/4, as
-          // scores of a model trained with its cap do, as x Q(x^2), an odd polynomial
-          // of u of degree 11 with the least largest error of tanh on [0, 3/4] (1.3e-8,
-          // fitted for this kernel; of degree 7 below 0.35: 8.8e-9), cap and scale in
-          // its coefficients: 7 (5) multiply-adds a score. Else cap - 2 cap / (1 +
-          // exp(2 u)), two more results of the exponential unit, which bounds the
-          // softmax. (Multiplying out u, u^2 and v apart took 10, and the FMA pipe
-          // 2300 cycles a tile and warp against 1400 for the rest.)
+          // scores of a model trained with its cap do, as u Q(u^2), an odd polynomial of
+          // degree 11 fitted for this kernel to tanh on [0, 3/4] (of degree 7 below 0.35),
+          // the cap in its coefficients: 8 (6) operations a score, two scores at a time.
+          // Else cap - 2 cap / (1 + exp(2 u)), two more results of the exponential unit,
+          // which bounds the softmax. (u is formed, for one operation more than a
+          // polynomial of x takes: that one's coefficients hold the tenth power of
+          // scale / cap, which 32 bits lose below 1e-4 and above 1e3.)
           float big = 0.f;
+          const uint64_t cap_u = pair_of(p.cap_u, p.cap_u);
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int e = 0; e < 32; e += 2)
-              big = fmax3_abs(big, __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-          const float most = big * p.cap_u;
-          const float u2 = p.cap_u * p.cap_u;
-          auto both = [](float x) { return pair_of(x, x); };
-          auto odd = [&](auto terms, float c1, float c2, float c3, float c4, float c5) {
-            const uint64_t k0 = both(p.scale_log2), k1 = both(c1 * u2 * p.scale_log2),
-                           k2 = both(c2 * u2 * u2 * p.scale_log2),
-                           k3 = both(c3 * u2 * u2 * u2 * p.scale_log2),
-                           k4 = both(c4 * u2 * u2 * (u2 * u2) * p.scale_log2),
-                           k5 = both(c5 * u2 * u2 * (u2 * u2) * u2 * p.scale_log2);
+            for (int e = 0; e < 32; e += 2) {
+              const float2 u = pair_floats(
+                  mul2(pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), cap_u));
+              s[c][e] = __float_as_uint(u.x);
+              s[c][e + 1] = __float_as_uint(u.y);
+              big = fmax3_abs(big, u.x, u.y);
+            }
+          auto odd = [&](auto coef) {
+            constexpr int N = sizeof(coef.c) / sizeof(float);
+            uint64_t k[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) k[i] = pair_of(coef.c[i] * p.cap_log2, coef.c[i] * p.cap_log2);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
               for (int e = 0; e < 32; e += 2) {
-                const uint64_t x = pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-                const uint64_t t = mul2(x, x);
-                uint64_t q = k3;
-                if constexpr (decltype(terms)::value == 5) q = fma2(t, fma2(t, k5, k4), k3);
-                q = fma2(t, fma2(t, fma2(t, q, k2), k1), k0);
-                const uint64_t y = mul2(x, q);
-                asm("mov.b64 {%0, %1}, %2;" : "=r"(s[c][e]), "=r"(s[c][e + 1]) : "l"(y));
+                const uint64_t u = pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+                const uint64_t t = mul2(u, u);
+                uint64_t q = k[N - 1];
+#pragma unroll
+                for (int i = N - 2; i >= 0; --i) q = fma2(t, q, k[i]);
+                const float2 y = pair_floats(mul2(u, q));
+                s[c][e] = __float_as_uint(y.x);
+                s[c][e + 1] = __float_as_uint(y.y);
               }
           };
-          if (__all_sync(0xffffffffu, most < 0.35f)) {
-            odd(std::integral_constant<int, 3>{}, -0.3333243131637573f, 0.13294382393360138f,
-                -0.04885116592049599f, 0.f, 0.f);
-          } else if (__all_sync(0xffffffffu, most < 0.75f)) {
-            odd(std::integral_constant<int, 5>{}, -0.33332908153533936f, 0.13324248790740967f,
-                -0.05328230932354927f, 0.01945533975958824f, -0.004626113455742598f);
+          if (__all_sync(0xffffffffu, big < 0.35f)) {
+            odd(TanhLow{});
+          } else if (__all_sync(0xffffffffu, big < 0.75f)) {
+            odd(TanhMid{});
           } else {
-            const float arg = 2.f * 1.4426950408889634f * p.cap_u;
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                s[c][e] = __float_as_uint(fmaf(
-                    -2.f * p.cap_log2, fast_rcp(1.f + fast_exp2(__uint_as_float(s[c][e]) * arg)),
-                    p.cap_log2));
+                s[c][e] = __float_as_uint(tanh_far(__uint_as_float(s[c][e]), p.cap_log2));
           }
         }
         if constexpr (MOD & 2) {

@@ -1357,8 +1357,11 @@ int bc_chunk_attention(const bc_shape* s, int tokens, int dtype, const void* q,
   p.out = output;
   p.out_f32 = output_f32;
   p.scale_log2 = options->scale * kLog2e;
-  p.cap_log2 = options->softcap * kLog2e;
-  p.cap_u = options->softcap > 0.f ? options->scale / options->softcap : 0.f;
+  // (a cap beyond 2^126 caps no score; where scale / cap would overflow, a score is 0 or
+  // at the cap either way)
+  const float cap = std::min(options->softcap, 8.5070592e37f);
+  p.cap_log2 = cap * kLog2e;
+  p.cap_u = cap > 0.f ? std::min(options->scale / cap, 3.4028235e38f) : 0.f;
   p.part_rows = plan.rows;
   if (plan.bytes > 0) {
     p.part_o = static_cast<float4*>(workspace);

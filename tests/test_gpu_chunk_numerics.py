@@ -1,12 +1,12 @@
-"""chunk_attention where its arithmetic can go wrong: infinities and NaN in what
-a row sees."""
+"""chunk_attention where its arithmetic can go wrong: score caps from tiny to
+huge, infinities and NaN in what a row sees."""
 import math
 
 import pytest
 import torch
 
 import serving_oracle as S
-from test_gpu_chunk_attention import BF16, F16, make
+from test_gpu_chunk_attention import BF16, F16, check, make
 
 pytestmark = pytest.mark.gpu
 
@@ -18,6 +18,64 @@ def bc():
     import branchcraft_torch
 
     return branchcraft_torch
+
+
+# ------------------------------------------------------------------ score caps
+
+
+def two_keys(scale, softcap, most, dtype, dim=128):
+    """64 heads of one token that sees two keys. Key 1, the token's own, has score 0; head
+    h's score with key 0 is near softcap * tanh(u_h), |u_h| <= most, and its distance bias
+    takes about as much off: the output weighs what is left."""
+    u = torch.cat([torch.linspace(-1, 1, 58), torch.tensor([0, 1e-6, -1e-6, 1e-3, -1e-3, 0.02])])
+    u = u.double() * most
+    q = (u * softcap / scale / dim).to(dtype)[None, :, None].expand(1, 64, dim).contiguous()
+    k = torch.zeros(1, 16, 1, dim, dtype=dtype)
+    k[0, 0] = 1
+    v = torch.zeros(1, 16, 1, dim, dtype=dtype)
+    v[0, 0], v[0, 1] = 1, -1
+    score = softcap * torch.tanh(q[0, :, 0].double() * dim * scale / softcap)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    f = dict(q=q.cuda(), k=k.cuda(), v=v.cuda(), pages=ints([[0]]), query_start=ints([0, 1]),
+             lengths=ints([2]))
+    return f, score.float().cuda()
+
+
+@pytest.mark.parametrize("dtype,scale,softcap", [
+    (F16, 0.0884, 0.5), (F16, 0.0884, 50.0), (BF16, 0.0884, 50.0), (BF16, 0.001, 50.0),
+    (F16, 0.0884, 3000.0), (BF16, 0.0884, 1e4), (BF16, 1e-5, 1.0),
+    (BF16, 1.0, 1e-4), (BF16, 1.0, 1e-7), (BF16, 1e-3, 1e-30)])
+@pytest.mark.parametrize("most", [0.34, 0.745, 4.0])
+def test_cap_of_any_size(bc, dtype, scale, softcap, most):
+    f, score = two_keys(scale, softcap, most, dtype)
+    got = check(bc, f, out_dtype=torch.float32, scale=scale, softcap=softcap, alibi_slopes=score)
+    # q.k is exact here (128 equal terms of at most 11 bits), so the score is off by its own
+    # arithmetic alone: some eight roundings of 2^-24 of the cap, the polynomial's 2^-26, and
+    # 2^-22 for each approximate unit: below 2^-19 of the cap. The output is tanh(x / 2) of
+    # what is left, whose slope is 1/2 at most.
+    want = S.chunk_attention(**f, scale=scale, softcap=softcap, alibi_slopes=score)[0]
+    tol = 2.0 ** -20 * softcap + torch.finfo(dtype).eps / 2 + 2.0 ** -16
+    assert ((got.cpu().double() - want).abs() <= tol).all()
+    # the same scores without the bias, and rows of zeros
+    check(bc, f, scale=scale, softcap=softcap)
+    f["q"].zero_()
+    f["v"].fill_(1)
+    check(bc, f, scale=scale, softcap=softcap)
+
+
+@pytest.mark.parametrize("softcap", [1e3, 1e5, 1e10, 1e25, 3e38])
+def test_wide_caps_leave_scores(bc, softcap):
+    """A cap far beyond the scores: what there is without one (softcap * tanh(x / softcap)
+    is x but for (x / softcap)^2 / 3, 1e-5 at most here)."""
+    f = make([50, 1], [300, 700], 6, 2, 128, F16, seed=21)
+    check(bc, f, softcap=softcap)
+
+
+@pytest.mark.parametrize("softcap", [1e-3, 1e-10, 1e-38, 1e-45])
+def test_narrow_caps_leave_the_mean(bc, softcap):
+    f = make([50, 1], [300, 700], 6, 2, 128, F16, seed=22)
+    f["q"][7] = 0
+    check(bc, f, softcap=softcap)
 
 
 # ------------------------------------------------- values that are not finite
