@@ -57,6 +57,15 @@ constexpr int kChLaunchRegs = 168, kChSoftmaxRegs = 208, kChOtherRegs = 88;
 static_assert(256 * kChSoftmaxRegs + 128 * kChOtherRegs == kChThreads * kChLaunchRegs,
               "the register split must use exactly the launch budget");
 
+// softcap tanh(x scale / softcap) of a score x, in log2 units: with x' = x pre, x' times a
+// polynomial of x'^2 while |x'| < near, else by its exponential. pre is 1 where the
+// coefficients, whose last holds the eighth power of scale / softcap, are ordinary
+// numbers; elsewhere it is scale / softcap itself, for one multiplication more.
+struct ChunkCap {
+  float k[5];
+  float near, arg, log2, pre;
+};
+
 struct ChunkParams {
   int batch, tokens, hq, hkv, group;
   int tile_tokens;            // tokens of a row tile: 128 / group
@@ -72,7 +81,7 @@ struct ChunkParams {
   void* out;                  // [tokens, hq, D]
   int out_f32;
   float scale_log2;           // scale * log2(e)
-  float cap_log2, cap_u;      // softcap * log2(e), scale / softcap, both finite
+  ChunkCap cap;               // (used with a cap)
   // workspace of split items (null when none can be split)
   float4* part_o;             // [blocks * 2][D / 4][part_rows]
   float2* part_ml;            // [blocks * 2][part_rows]
@@ -248,18 +257,6 @@ __device__ __forceinline__ void add_pair(float& a0, float& a1, float b0, float b
       "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
       : "+f"(a0), "+f"(a1)
       : "f"(b0), "f"(b1));
-}
-
-// tanh(u) / u in powers of u^2: up to |u| = 0.35, and up to 3/4.
-struct TanhLow {
-  float c[4] = {1.f, -0.3333243131637573f, 0.13294382393360138f, -0.04885116592049599f};
-};
-struct TanhMid {
-  float c[6] = {1.f, -0.33332908153533936f, 0.13324248790740967f, -0.05328230932354927f,
-                0.01945533975958824f, -0.004626113455742598f};
-};
-__device__ __forceinline__ float tanh_far(float u, float cap) {
-  return fmaf(-2.f * cap, fast_rcp(1.f + fast_exp2(u * (2.f * 1.4426950408889634f))), cap);
 }
 
 // Largest magnitude of three.
@@ -845,55 +842,55 @@ __global__ void __launch_bounds__(kChThreads, 1)
         // Scores in log2 units when they are capped or biased; otherwise the
         // scale (> 0) waits for the exponent's multiply-add.
         if constexpr (MOD & 1) {
-          // cap * tanh(u), u = x scale / cap. While the warp's |u| stay below 3/4, as
-          // scores of a model trained with its cap do, as u Q(u^2), an odd polynomial of
-          // degree 11 fitted for this kernel to tanh on [0, 3/4] (of degree 7 below 0.35),
-          // the cap in its coefficients: 8 (6) operations a score, two scores at a time.
-          // Else cap - 2 cap / (1 + exp(2 u)), two more results of the exponential unit,
-          // which bounds the softmax. (u is formed, for one operation more than a
-          // polynomial of x takes: that one's coefficients hold the tenth power of
-          // scale / cap, which 32 bits lose below 1e-4 and above 1e3.)
-          float big = 0.f;
-          const uint64_t cap_u = pair_of(p.cap_u, p.cap_u);
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 u = pair_floats(
-                  mul2(pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), cap_u));
-              s[c][e] = __float_as_uint(u.x);
-              s[c][e + 1] = __float_as_uint(u.y);
-              big = fmax3_abs(big, u.x, u.y);
-            }
-          auto odd = [&](auto coef) {
-            constexpr int N = sizeof(coef.c) / sizeof(float);
-            uint64_t k[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) k[i] = pair_of(coef.c[i] * p.cap_log2, coef.c[i] * p.cap_log2);
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                const uint64_t u = pair_of(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-                const uint64_t t = mul2(u, u);
-                uint64_t q = k[N - 1];
-#pragma unroll
-                for (int i = N - 2; i >= 0; --i) q = fma2(t, q, k[i]);
-                const float2 y = pair_floats(mul2(u, q));
-                s[c][e] = __float_as_uint(y.x);
-                s[c][e + 1] = __float_as_uint(y.y);
-              }
-          };
-          if (__all_sync(0xffffffffu, big < 0.35f)) {
-            odd(TanhLow{});
-          } else if (__all_sync(0xffffffffu, big < 0.75f)) {
-            odd(TanhMid{});
-          } else {
+          // cap * tanh(u), u = x scale / cap, by the score's own size, so that no other
+          // score changes a bit of it: below |u| = 0.55, where scores of a model trained
+          // with its cap lie, as x Q(x^2), an odd polynomial of u of degree 9 (ChunkCap),
+          // 6 operations a score, two scores at a time; beyond as
+          // cap - 2 cap / (1 + exp(2 u)), two more results of the exponential unit, which
+          // bounds the softmax. A warp without such scores skips that form.
+          if (p.cap.pre != 1.f) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                s[c][e] = __float_as_uint(tanh_far(__uint_as_float(s[c][e]), p.cap_log2));
+                s[c][e] = __float_as_uint(__uint_as_float(s[c][e]) * p.cap.pre);
+          }
+          float big = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+              big = fmax3_abs(big, __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+          auto both = [](float x) { return pair_of(x, x); };
+          const uint64_t k0 = both(p.cap.k[0]), k1 = both(p.cap.k[1]), k2 = both(p.cap.k[2]),
+                         k3 = both(p.cap.k[3]), k4 = both(p.cap.k[4]);
+          auto near = [&](float x0, float x1) -> float2 {
+            const uint64_t x = pair_of(x0, x1), t = mul2(x, x);
+            return pair_floats(mul2(x, fma2(t, fma2(t, fma2(t, fma2(t, k4, k3), k2), k1), k0)));
+          };
+          if (__all_sync(0xffffffffu, big < p.cap.near)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float2 y = near(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+                s[c][e] = __float_as_uint(y.x);
+                s[c][e + 1] = __float_as_uint(y.y);
+              }
+          } else {
+            auto far = [&](float x) {
+              return fmaf(-2.f * p.cap.log2, fast_rcp(1.f + fast_exp2(x * p.cap.arg)), p.cap.log2);
+            };
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float x0 = __uint_as_float(s[c][e]), x1 = __uint_as_float(s[c][e + 1]);
+                const float2 y = near(x0, x1);
+                s[c][e] = __float_as_uint(fabsf(x0) < p.cap.near ? y.x : far(x0));
+                s[c][e + 1] = __float_as_uint(fabsf(x1) < p.cap.near ? y.y : far(x1));
+              }
+            __syncwarp();
           }
         }
         if constexpr (MOD & 2) {

@@ -1137,6 +1137,29 @@ struct ChunkPlan {
   }
 };
 
+// tanh(u) / u in powers of u^2 up to |u| = kTanhNear, fitted for the smallest largest
+// error of tanh there: 1.2e-8 with these coefficients.
+constexpr double kTanh[5] = {1.0, -0.33332759141921997, 0.13317517936229706, -0.05250634625554085,
+                             0.016171788796782494};
+constexpr double kTanhNear = 0.55;
+
+ChunkCap chunk_cap(double scale, double softcap) {
+  const double u = scale / softcap;  // of a score of 1
+  const bool fold = u > 1e-4 && u < 1e4 && scale > 1e-5 && scale < 1e5;
+  // (a cap beyond 2^126 caps no score, and with such a u a score is 0 or at the cap: both
+  // stay within 32 bits)
+  const double most = 8.5e37, cap = std::min(softcap, most), log2e = 1.4426950408889634;
+  const double x = fold ? u : 1.0;
+  ChunkCap c;
+  double power = (fold ? scale : cap) * log2e;
+  for (int i = 0; i < 5; ++i, power *= x * x) c.k[i] = float(kTanh[i] * power);
+  c.near = float(kTanhNear / x);
+  c.arg = float(2.0 * log2e * x);
+  c.log2 = float(cap * log2e);
+  c.pre = fold ? 1.f : float(std::min(scale / cap, most));
+  return c;
+}
+
 template <int D, typename T, int MOD>
 cudaError_t launch_chunk_mod(ChunkParams& p, const CUtensorMap* maps, const ChunkPlan& plan,
                              int dev, cudaStream_t stream) {
@@ -1357,11 +1380,7 @@ int bc_chunk_attention(const bc_shape* s, int tokens, int dtype, const void* q,
   p.out = output;
   p.out_f32 = output_f32;
   p.scale_log2 = options->scale * kLog2e;
-  // (a cap beyond 2^126 caps no score; where scale / cap would overflow, a score is 0 or
-  // at the cap either way)
-  const float cap = std::min(options->softcap, 8.5070592e37f);
-  p.cap_log2 = cap * kLog2e;
-  p.cap_u = cap > 0.f ? std::min(options->scale / cap, 3.4028235e38f) : 0.f;
+  if (options->softcap > 0.f) p.cap = chunk_cap(options->scale, options->softcap);
   p.part_rows = plan.rows;
   if (plan.bytes > 0) {
     p.part_o = static_cast<float4*>(workspace);

@@ -1,5 +1,6 @@
 """chunk_attention where its arithmetic can go wrong: score caps from tiny to
-huge, infinities and NaN in what a row sees."""
+huge, bits that must not depend on what a row does not see, infinities and NaN
+in what it does see."""
 import math
 
 import pytest
@@ -18,6 +19,63 @@ def bc():
     import branchcraft_torch
 
     return branchcraft_torch
+
+
+# ------------------------------------------------------- bits and unseen values
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("softcap", [4.0, 30.0])
+@pytest.mark.parametrize("bad", [60.0, INF, -INF, NAN])
+def test_unseen_keys_change_no_capped_bit(bc, dtype, softcap, bad):
+    """Slots past the lengths, pages that no token sees and keys that only later
+    tokens see, with scores capped and seven heads a group (126 of 128 rows used)."""
+    f = make([60, 1], [200, 1000], 14, 2, 128, dtype, seed=7)
+    want = bc.chunk_attention(**f, window=130, softcap=softcap)
+    g = dict(f, k=f["k"].clone(), v=f["v"].clone())
+    used = torch.zeros(f["k"].shape[0], 16, dtype=torch.bool)
+    for b, (n, x) in enumerate(((60, 200), (1, 1000))):
+        for j in range(max(0, x - n + 1 - 130), x):
+            used[int(f["pages"][b, j // 16]), j % 16] = True
+    for name in ("k", "v"):
+        g[name][~used.cuda()] = bad
+    assert torch.equal(bc.chunk_attention(**g, window=130, softcap=softcap), want)
+    k = f["k"].clone()
+    k[int(f["pages"][0, 199 // 16]), 199 % 16] = bad
+    got = bc.chunk_attention(**dict(f, k=k), window=130, softcap=softcap)
+    assert torch.equal(got[:59], want[:59]) and torch.equal(got[60:], want[60:])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_other_requests_change_no_capped_bit(bc, dtype):
+    """A request's last row tile also holds the next request's rows."""
+    f = make([20, 41], [300, 41], 14, 2, 128, dtype, seed=8)
+    want = bc.chunk_attention(**f, softcap=30.0)
+    q = f["q"].clone()
+    q[20:] *= 60
+    got = bc.chunk_attention(**dict(f, q=q), softcap=30.0)
+    assert torch.equal(got[:20], want[:20])
+    # one row's scores do not change the next row's
+    q = f["q"].clone()
+    q[3, 5] *= 60
+    got = bc.chunk_attention(**dict(f, q=q), softcap=30.0)
+    same = torch.ones(61, 14, dtype=torch.bool, device="cuda")
+    same[3, 5] = False
+    assert torch.equal(got[same], want[same])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_earlier_calls_change_no_capped_bit(bc, dtype):
+    """With seven heads a group two rows of a tile are nobody's: what an earlier
+    launch left in their place is not looked at."""
+    f = make([18], [300], 7, 1, 128, dtype, seed=9)
+    calm = make([2500], [2500], 8, 1, 128, dtype, seed=10)
+    wild = dict(calm, q=calm["q"] * 100)
+    got = []
+    for before in (calm, wild, calm, wild):
+        bc.chunk_attention(**before, softcap=30.0)
+        got.append(bc.chunk_attention(**f, softcap=30.0))
+    assert all(torch.equal(x, got[0]) for x in got)
 
 
 # ------------------------------------------------------------------ score caps
@@ -43,7 +101,7 @@ def two_keys(scale, softcap, most, dtype, dim=128):
 
 @pytest.mark.parametrize("dtype,scale,softcap", [
     (F16, 0.0884, 0.5), (F16, 0.0884, 50.0), (BF16, 0.0884, 50.0), (BF16, 0.001, 50.0),
-    (F16, 0.0884, 3000.0), (BF16, 0.0884, 1e4), (BF16, 1e-5, 1.0),
+    (F16, 0.0884, 3000.0), (BF16, 0.0884, 1e4), (F16, 0.0884, 1e5), (BF16, 1e-5, 1.0),
     (BF16, 1.0, 1e-4), (BF16, 1.0, 1e-7), (BF16, 1e-3, 1e-30)])
 @pytest.mark.parametrize("most", [0.34, 0.745, 4.0])
 def test_cap_of_any_size(bc, dtype, scale, softcap, most):

@@ -201,3 +201,19 @@ def test_append_refuses_rows_before_it_plans(monkeypatch):
             seq.append(good, bad, new)
     with pytest.raises(AssertionError):
         seq.append(good, good, new)
+
+
+def test_tanh_polynomial_error():
+    """The coefficients and their error as the source states them."""
+    import re
+    from pathlib import Path
+
+    import numpy as np
+
+    text = (Path(C.__file__).parent / "csrc" / "branchcraft.cu").read_text()
+    coef = [float(x) for x in re.search(r"kTanh\[5\] = \{([^}]*)\}", text)[1].split(",")]
+    border = float(re.search(r"kTanhNear = ([\d.]+)", text)[1])
+    stated = float(re.search(r"error of tanh there: (\S+) with these", text)[1])
+    u = np.linspace(0, border, 200001)
+    err = np.abs(u * sum(c * u ** (2 * i) for i, c in enumerate(coef)) - np.tanh(u)).max()
+    assert 0.9 * stated < err <= 1.01 * stated
