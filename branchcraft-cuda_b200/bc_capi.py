@@ -381,9 +381,21 @@ def last_device_error(reset: bool = True) -> int:
 DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
-def kv_layout(cache) -> KvLayout:
-    """The strides of a cache (or a view of one) shaped [P, 16, Hkv, D]."""
+def kv_layout(cache, other=None) -> KvLayout:
+    """The strides of a cache (or a view of one) shaped [P, 16, Hkv, D], which `other`
+    (V beside K) has to share."""
+    if cache.dim() != 4 or cache.stride(3) != 1:
+        raise ValueError("a cache is [P, 16, Hkv, D] with a contiguous last dimension")
+    if other is not None and (other.shape != cache.shape or other.stride() != cache.stride()):
+        raise ValueError("K and V caches must have equal shapes and strides")
     return KvLayout(cache.stride(0), cache.stride(1), cache.stride(2))
+
+
+def _rows(t, name):
+    """Elements between the tokens of [tokens, heads, D], each token's heads contiguous."""
+    if t.dim() != 3 or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError(f"{name} must be [tokens, heads, D], each token's heads contiguous")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
 
 class AppendPlan:
@@ -420,9 +432,9 @@ def append_plan(pages, lengths, new_tokens, state, plan: AppendPlan, state_out=N
 def append_kv(shape: Shape, k, v, cache_k, cache_v, slot_map, clones=None, counts=None,
               stream=None):
     """k, v [tokens, Hkv, D] into the cache rows slot_map names, and a plan's clones."""
-    layout = kv_layout(cache_k)
-    _check(_lib.bc_append_kv(ctypes.byref(shape), k.shape[0], _ptr(k), k.stride(0), _ptr(v),
-                             v.stride(0), _ptr(cache_k), _ptr(cache_v), ctypes.byref(layout),
+    layout = kv_layout(cache_k, cache_v)
+    _check(_lib.bc_append_kv(ctypes.byref(shape), k.shape[0], _ptr(k), _rows(k, "k"), _ptr(v),
+                             _rows(v, "v"), _ptr(cache_k), _ptr(cache_v), ctypes.byref(layout),
                              _ptr(slot_map), _ptr(clones),
                              0 if clones is None else clones.shape[1],
                              None if counts is None else ctypes.c_void_p(counts.data_ptr() + 4),
@@ -442,9 +454,9 @@ def chunk_attention(shape: Shape, q, cache_k, cache_v, pages, query_start, lengt
 
     options = ChunkOptions(scale if scale is not None else shape.dim ** -0.5, softcap, window,
                            dev(alibi_slopes), dev(prefix), dev(key_start))
-    layout = kv_layout(cache_k)
+    layout = kv_layout(cache_k, cache_v)
     rc = _lib.bc_chunk_attention(ctypes.byref(shape), q.shape[0], DTYPES[q.dtype], _ptr(q),
-                                 q.stride(0), _ptr(cache_k), _ptr(cache_v), ctypes.byref(layout),
+                                 _rows(q, "q"), _ptr(cache_k), _ptr(cache_v), ctypes.byref(layout),
                                  _ptr(pages), _ptr(query_start), _ptr(lengths),
                                  ctypes.byref(options), _ptr(output),
                                  int(output.dtype == torch.float32), _ptr(workspace),
@@ -461,8 +473,11 @@ def beam_workspace_bytes(batch, beams, vocab, k, dtype) -> int:
 def beam_select(logits, scores, k, out_scores, out_tokens, out_parents, workspace, stream=None):
     """logits [batch, beams, vocab], scores [batch, beams]; outputs [batch, k]."""
     batch, beams, vocab = logits.shape
+    stride = logits.stride(1) if beams > 1 else logits.stride(0) if batch > 1 else vocab
+    if (vocab > 1 and logits.stride(2) != 1) or (batch > 1 and logits.stride(0) != beams * stride):
+        raise ValueError("logits' rows must be contiguous and equally far apart")
     _check(_lib.bc_beam_select(batch, beams, vocab, k, DTYPES[logits.dtype], _ptr(logits),
-                               logits.stride(1), _ptr(scores), _ptr(out_scores),
+                               stride, _ptr(scores), _ptr(out_scores),
                                _ptr(out_tokens), _ptr(out_parents), _ptr(workspace),
                                workspace.numel(), _stream(stream)), "bc_beam_select")
 

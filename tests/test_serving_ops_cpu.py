@@ -217,3 +217,62 @@ def test_tanh_polynomial_error():
     u = np.linspace(0, border, 200001)
     err = np.abs(u * sum(c * u ** (2 * i) for i, c in enumerate(coef)) - np.tanh(u)).max()
     assert 0.9 * stated < err <= 1.01 * stated
+
+
+class Recorder:
+    """Stands in for the library: keeps a call's arguments, reports success."""
+
+    def __init__(self):
+        self.args = None
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.args = args
+            return 0
+        return call
+
+
+def test_capi_strides_of_views(monkeypatch):
+    """What the ctypes wrappers take as the distance of rows, and the views they refuse."""
+    rec = Recorder()
+    monkeypatch.setattr(C, "_lib", rec)
+    monkeypatch.setattr(C, "_stream", lambda s=None: None)
+    wide = torch.zeros(3, 4, 50)
+    out = torch.zeros(3, 2)
+
+    def select(x):
+        C.beam_select(x, torch.zeros(x.shape[:2]), 2, out, out.int(), out.int(), out)
+        return rec.args[6]
+
+    assert select(wide) == 50
+    assert select(wide[:, :1]) == 200   # one beam of every request
+    assert select(wide[1:2, :2]) == 50
+    assert select(wide[:, :, :40]) == 50
+    for bad in (wide[:, :2], wide[:, ::2][:, :1].expand(3, 2, 50), wide[..., ::2],
+                wide.transpose(0, 1), torch.zeros(3, 50, 4).transpose(1, 2)):
+        with pytest.raises(ValueError):
+            select(bad)
+
+    cache = torch.zeros(5, 16, 2, 64, dtype=torch.float16)
+    planes = torch.zeros(5, 2, 16, 2, 64, dtype=torch.float16)
+    q = torch.zeros(3, 8, 64, dtype=torch.float16)
+    i = torch.zeros(4, dtype=torch.int32)
+    s = shape(physical_pages=5)
+
+    def both(k, v, x=q):
+        C.chunk_attention(s, x, k, v, i, i, i, q)
+        chunk = rec.args[4]
+        C.append_kv(s, x[:, :2], x[:, :2], k, v, i)
+        assert rec.args[3] == rec.args[5] == chunk
+        return chunk
+
+    assert both(planes[:, 0], planes[:, 1]) == 512
+    assert both(cache, cache, torch.zeros(3, 12, 64, dtype=torch.float16)[:, :8]) == 768
+    for k, v in ((cache, planes[:, 1]), (planes[:, 0], cache), (cache, cache[:4]),
+                 (cache[..., ::2], cache[..., ::2])):
+        with pytest.raises(ValueError):
+            both(k, v)
+    for x in (torch.zeros(3, 8, 128, dtype=torch.float16)[..., :64],
+              torch.zeros(8, 3, 64, dtype=torch.float16).transpose(0, 1)):
+        with pytest.raises(ValueError):
+            both(cache, cache, x)
