@@ -945,7 +945,10 @@ __global__ void __launch_bounds__(kChThreads, 1)
         ++sc;
         tc_fence_after();
         // Lazy maximum: the reference moves only when a row's maximum grows by
-        // more than 2^8, with probabilities up to 2^8 until then.
+        // more than 2^8, with probabilities up to 2^8 until then. FP16 ones (and with
+        // them l and O) are held times 2^7, up to 2^15: without it those below 2^-25 of
+        // the largest were rounded to 0, and of tens of thousands of keys such ones can
+        // make a thousandth of the output.
         float alpha = 1.f;
         bool rescale = false;
         if (mx > m_ref + 8.f) {
@@ -969,7 +972,8 @@ __global__ void __launch_bounds__(kChThreads, 1)
           }
           tmem_st_wait();
         }
-        const float mb = m_ref == kNegInf ? 0.f : -m_ref;
+        constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
+        const float mb = m_ref == kNegInf ? 0.f : kLift - m_ref;
         float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {

@@ -1,6 +1,6 @@
 """chunk_attention where its arithmetic can go wrong: score caps from tiny to
 huge, bits that must not depend on what a row does not see, infinities and NaN
-in what it does see."""
+in what it does see, and probabilities far below the largest one."""
 import math
 
 import pytest
@@ -218,3 +218,29 @@ def test_scores_of_minus_infinity(bc, new, length, ends, dtype, dim):
         f["k"][f["pages"][0, j // 16].item(), j % 16, :, 5] = -INF
     got = check_natural(bc, f)
     assert got.isnan().any() == (length - new < ends)
+
+
+# --------------------------------------------------------- small probabilities
+
+
+@pytest.mark.parametrize("new,batch,length", [(1, 160, 60000), (100, 40, 20000)])
+def test_many_small_probabilities(bc, new, batch, length):
+    """One key of score 18 and tens of thousands of score 0, 2^-26 of its weight each and a
+    thousandth of the output together. FP16 probabilities that small are rounded to
+    2^-25 2^-7 of the largest one (its smallest step, at the kernel's scale of 2^7). All
+    requests hold the same pages: enough of them that items are hardly split."""
+    f = make([new], [length], 8, 1, 128, F16, seed=41)
+    f["q"].fill_(18 / 128 ** 0.5)
+    f["k"].zero_()
+    f["v"].fill_(1)
+    first = f["pages"][0, 0].item()
+    f["k"][first, 0] = 1
+    f["v"][first, 0] = 0
+    got = bc.chunk_attention(
+        f["q"].repeat(batch, 1, 1), f["k"], f["v"], f["pages"].repeat(batch, 1),
+        torch.arange(batch + 1, dtype=torch.int32, device="cuda") * new, f["lengths"].repeat(batch))
+    got = got.cpu().double().view(batch, new, 8, 128)
+    want, spread, big = S.chunk_attention(**f)
+    u = 2.0 ** -11
+    tol = u * want + spread * (u + 2 * 136 * 2.0 ** -23 * big + 2.0 ** -16) + length * 2.0 ** -32
+    assert (want > 2e-4).all() and ((got - want).abs() <= tol).all()
