@@ -215,6 +215,14 @@ __device__ __forceinline__ float fast_rcp(float x) {
 }
 
 template <typename T>
+__device__ __forceinline__ float2 unpack_pair(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value)
+    return unpack_half2(w);
+  else
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+template <typename T>
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
   uint32_t r;
   if constexpr (std::is_same<T, __half>::value)
@@ -275,14 +283,17 @@ __device__ __forceinline__ void st_global_v8(void* to, uint32_t a, uint32_t b, u
                : "memory");
 }
 
-// MOD: bit 0 the tanh cap, bit 1 the distance bias.
-template <int D, typename T, int MOD>
+// MOD: bit 0 the tanh cap, bit 1 the distance bias. F32: FP32 output, whose
+// probabilities are held as two 16-bit numbers, handed over and multiplied one after
+// the other (P has no second place in TMEM).
+template <int D, typename T, int MOD, bool F32>
 __global__ void __launch_bounds__(kChThreads, 1)
     chunk_mma_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap qmap,
                      const __grid_constant__ CUtensorMap kmap,
                      const __grid_constant__ CUtensorMap vmap) {
   using G = ChunkGeom<D>;
   constexpr int KB = G::KB, NK = G::kKStages, NV = G::kVStages;
+  constexpr int kParts = F32 ? 2 : 1;  // of P
   constexpr float kNegInf = -INFINITY, kLowest = -3.402823466e38f;
   constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
   constexpr uint32_t kIdescS = umma_idesc_f16(128, kChTile, false, false) | kBf16;
@@ -676,14 +687,17 @@ __global__ void __launch_bounds__(kChThreads, 1)
 #pragma unroll 1
           for (int g = dual ? 0 : (j & 1); g <= (dual ? 1 : (j & 1)); ++g, ++count) {
             if (is_pv) {
-              const uint32_t par = (g ? pc[1] : pc[0]) & 1;
-              if (g) ++pc[1]; else ++pc[0];
               const uint64_t vd = vdesc + uint64_t((st * G::kRowTile) >> 4);
               const uint32_t acc = (dual ? j : j >> 1) > 0 ? 1u : 0u;
               // (the first half's products run while the second half of P is
               // still being made)
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
+              for (int i = 0; i < 2 * kParts; ++i) {
+                const int part = i >> 1, h = i & 1;
+                const uint32_t par = (g ? pc[1] : pc[0]) & 1;
+                if (h) {
+                  if (g) ++pc[1]; else ++pc[0];
+                }
                 ok = __all_sync(0xffffffffu, mbar_wait(h ? &p_full[g] : &p_half[g], par));
                 if (!ok) break;
                 tc_fence_after();
@@ -692,10 +706,10 @@ __global__ void __launch_bounds__(kChThreads, 1)
                   for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
                     umma_f16_ts(tbase + G::kTmemO + g * 128, tbase + G::kTmemP + g * 64 + kk * 8,
                                 vd + uint64_t((kk * 2 * G::kGroupBytes) >> 4), kIdescPV,
-                                kk > 0 ? 1u : acc);
+                                kk > 0 || part > 0 ? 1u : acc);
                   if (h) {
                     umma_commit(&p_done[g]);
-                    if (!dual || g == 1) umma_commit(&v_empty[st]);
+                    if (part == kParts - 1 && (!dual || g == 1)) umma_commit(&v_empty[st]);
                   }
                 }
                 __syncwarp();
@@ -765,6 +779,12 @@ __global__ void __launch_bounds__(kChThreads, 1)
     const uint32_t tO = tbase + lane_addr + G::kTmemO + uint32_t(grp) * 128;
     const int row_tok = row / p.group, row_head = row % p.group;
     uint32_t sc = 0, alt = 0;  // tiles of this group, ALT items done
+    uint32_t pn = 0;           // P handed over, where that is not one a tile
+    // The last P handed over has been multiplied: P is free, O holds its product.
+    auto p_taken = [&]() -> bool {
+      const uint32_t n = F32 ? pn : sc;
+      return n == 0 || __all_sync(0xffffffffu, mbar_wait(&p_done[grp], (n - 1) & 1));
+    };
     unsigned tile0 = 0;        // the item's first tile in the rings
     for (int k = 0; ok; ++k) {
       const int ds = k % kChDescs;
@@ -815,12 +835,14 @@ __global__ void __launch_bounds__(kChThreads, 1)
           const int j = dual ? n : 2 * n + grp;
           ok = __all_sync(0xffffffffu, mbar_wait(&s_full[grp], sc & 1));
           if (ok && lane == 0) mbar_arrive(s_free);
-          if (ok && sc > 0) ok = __all_sync(0xffffffffu, mbar_wait(&p_done[grp], (sc - 1) & 1));
-          ok = ok && zero_pads(j, (d.t0 + j) * kChTile);
-          __syncwarp();
-          if (ok && lane == 0) {
-            mbar_arrive(&p_half[grp]);
-            mbar_arrive(&p_full[grp]);
+          ok = ok && p_taken() && zero_pads(j, (d.t0 + j) * kChTile);
+          for (int part = 0; part < kParts && ok; ++part, ++pn) {
+            if (part > 0) ok = p_taken();
+            __syncwarp();
+            if (ok && lane == 0) {
+              mbar_arrive(&p_half[grp]);
+              mbar_arrive(&p_full[grp]);
+            }
           }
         }
       }
@@ -939,8 +961,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
         }
         if constexpr (MOD == 0) mx *= p.scale_log2;  // -inf stays -inf
         // P of the last tile has been read, and O holds its product.
-        if (sc > 0) ok = __all_sync(0xffffffffu, mbar_wait(&p_done[grp], (sc - 1) & 1));
-        ok = ok && zero_pads(j, k0);
+        ok = p_taken() && zero_pads(j, k0);
         if (!ok) break;
         ++sc;
         tc_fence_after();
@@ -991,10 +1012,16 @@ __global__ void __launch_bounds__(kChThreads, 1)
             x3 = fast_exp2(x3);
             add_pair(l0, l1, x0, x1);
             add_pair(l2, l3, x2, x3);
-            // (P in the input's 16 bits: one rounding of half a step a term, the A
-            // operand's type; the sum l keeps the unrounded values)
+            // (P in the input's 16 bits, as the A operand of a product with V has to be:
+            // one rounding of half a step a term, no more than the output's own; the sum
+            // l keeps the unrounded values)
             ph[e / 2] = pack_pair<T>(x0, x1);
             ph[e / 2 + 1] = pack_pair<T>(x2, x3);
+            if constexpr (F32) {  // what the rounding took off (in the scores' place)
+              const float2 h0 = unpack_pair<T>(ph[e / 2]), h1 = unpack_pair<T>(ph[e / 2 + 1]);
+              s[c][e / 2] = pack_pair<T>(x0 - h0.x, x1 - h0.y);
+              s[c][e / 2 + 1] = pack_pair<T>(x2 - h1.x, x3 - h1.y);
+            }
           }
           tmem_st16(tP + c * 16, ph);
           if (c == 1) {
@@ -1009,12 +1036,33 @@ __global__ void __launch_bounds__(kChThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[grp]);
+        if constexpr (F32) {
+          ++pn;
+          ok = p_taken();
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pl[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) pl[e] = s[c][e];
+            tmem_st16(tP + c * 16, pl);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&p_half[grp]);
+            mbar_arrive(&p_full[grp]);
+          }
+          ++pn;
+        }
       }
       if (!ok) break;
       tile0 += unsigned(d.nt);
 
       // -------------------------------------------------------------- epilogue
-      if (sc > 0) ok = __all_sync(0xffffffffu, mbar_wait(&p_done[grp], (sc - 1) & 1));
+      ok = p_taken();
       if (!ok) break;
       tc_fence_after();
       // A row that saw keys, but no score above -inf: a reference of its own tells it
@@ -1078,7 +1126,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
               to[size_t(e / 4) * p.part_rows] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
           } else if (valid) {
             const size_t at = (size_t(d.first + tok) * p.hq + head) * D + c;
-            if (p.out_f32) {
+            if constexpr (F32) {
               float4* to = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
 #pragma unroll
               for (int e = 0; e < 32; e += 4)

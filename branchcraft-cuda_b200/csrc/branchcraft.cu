@@ -1160,10 +1160,10 @@ ChunkCap chunk_cap(double scale, double softcap) {
   return c;
 }
 
-template <int D, typename T, int MOD>
+template <int D, typename T, int MOD, bool F32>
 cudaError_t launch_chunk_mod(ChunkParams& p, const CUtensorMap* maps, const ChunkPlan& plan,
                              int dev, cudaStream_t stream) {
-  auto kern = chunk_mma_kernel<D, T, MOD>;
+  auto kern = chunk_mma_kernel<D, T, MOD, F32>;
   static std::atomic<size_t> smem_of[kMaxDevices];
   size_t smem = smem_of[dev].load(std::memory_order_relaxed);
   if (!smem) {
@@ -1187,15 +1187,22 @@ cudaError_t launch_chunk_mod(ChunkParams& p, const CUtensorMap* maps, const Chun
                           stream, p);
 }
 
+template <int D, typename T, bool F32>
+cudaError_t launch_chunk_out(ChunkParams& p, const CUtensorMap* maps, const ChunkPlan& plan,
+                         const bc_chunk_options* o, int dev, cudaStream_t stream) {
+  switch ((o->softcap > 0.f ? 1 : 0) | (o->alibi_slopes ? 2 : 0)) {
+    case 0: return launch_chunk_mod<D, T, 0, F32>(p, maps, plan, dev, stream);
+    case 1: return launch_chunk_mod<D, T, 1, F32>(p, maps, plan, dev, stream);
+    case 2: return launch_chunk_mod<D, T, 2, F32>(p, maps, plan, dev, stream);
+    default: return launch_chunk_mod<D, T, 3, F32>(p, maps, plan, dev, stream);
+  }
+}
+
 template <int D, typename T>
 cudaError_t launch_chunk(ChunkParams& p, const CUtensorMap* maps, const ChunkPlan& plan,
                          const bc_chunk_options* o, int dev, cudaStream_t stream) {
-  switch ((o->softcap > 0.f ? 1 : 0) | (o->alibi_slopes ? 2 : 0)) {
-    case 0: return launch_chunk_mod<D, T, 0>(p, maps, plan, dev, stream);
-    case 1: return launch_chunk_mod<D, T, 1>(p, maps, plan, dev, stream);
-    case 2: return launch_chunk_mod<D, T, 2>(p, maps, plan, dev, stream);
-    default: return launch_chunk_mod<D, T, 3>(p, maps, plan, dev, stream);
-  }
+  return p.out_f32 ? launch_chunk_out<D, T, true>(p, maps, plan, o, dev, stream)
+                   : launch_chunk_out<D, T, false>(p, maps, plan, o, dev, stream);
 }
 
 // Rows are cut into the number of segments that takes the least time by count:

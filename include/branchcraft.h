@@ -400,11 +400,12 @@ typedef struct bc_chunk_options {
  * (BC_F16 or BC_BF16) is that of q, k, v and, unless output_f32 != 0, of output
  * [tokens, query_heads, dim], contiguous; rows in no request are left as they
  * are. Sums are held in FP32; probabilities are rounded to dtype before the
- * product with V. Slots past a request's length and pages that none of its
- * tokens sees may hold anything; the values (V) of keys that some token of the
- * request sees must be finite. Malformed starts and lengths are brought into
- * range and set BC_ERR_LENGTH; a seen page outside the pool reads as zeros and
- * sets BC_ERR_PAGE_RANGE. query_heads / kv_heads at most 128; addresses and
+ * product with V, and for FP32 output held as two numbers of it. Slots past a
+ * request's length and pages that none of its tokens sees may hold anything; the
+ * values (V) of keys that some token of the request sees must be finite.
+ * Malformed starts and lengths are brought into range and set BC_ERR_LENGTH; a
+ * seen page outside the pool reads as zeros and sets BC_ERR_PAGE_RANGE.
+ * query_heads / kv_heads at most 128; addresses and
  * strides are multiples of 16 bytes, output's of 32, head_stride one of 64
  * elements; batch at most BC_MAX_CHUNK_REQUESTS.
  * workspace: bc_chunk_workspace_bytes, 16-byte aligned, one per call in

@@ -244,3 +244,52 @@ def test_many_small_probabilities(bc, new, batch, length):
     u = 2.0 ** -11
     tol = u * want + spread * (u + 2 * 136 * 2.0 ** -23 * big + 2.0 ** -16) + length * 2.0 ** -32
     assert (want > 2e-4).all() and ((got - want).abs() <= tol).all()
+
+
+# ----------------------------------------------------------------- FP32 output
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,lens,hq,hkv", [
+    ([1], [1], 1, 1), ([1, 1, 1], [1, 130, 1000], 8, 2), ([129], [640], 6, 2),
+    ([200, 1, 0, 37], [200, 900, 40, 37], 8, 2), ([7, 7], [200, 16], 14, 2), ([300], [300], 7, 1),
+    ([1, 3], [20000, 9001], 8, 2), ([700], [1800], 2, 1)])
+def test_fp32_output_keeps_probabilities(bc, new, lens, hq, hkv, dim, dtype):
+    """For FP32 output a probability is two 16-bit numbers: what the first rounds off, 2^-9
+    of it at most, the second holds to 2^-9 of that (2^-12 and 2^-24 for FP16): 2^-18
+    together, within assert_chunk_close's 2^-16 for the exponential; no rounding of 2^-9 or
+    2^-12 is left. Sixteen additions to the output a tile of 128 keys, of two products of
+    eight steps each, may cut 2^-23 of the sum."""
+    f = make(new, lens, hq, hkv, dim, dtype, seed=51)
+    for options in ({}, dict(softcap=20.0, window=300), dict(scale=0.3)):
+        got = torch.full(f["q"].shape, NAN, device="cuda")
+        bc.chunk_attention_out(*(f[n] for n in ("q", "k", "v", "pages", "query_start", "lengths")),
+                               got, **options)
+        want, spread, big = S.chunk_attention(**f, **options)
+        tiles = torch.tensor([(x + 127) // 128 for n, x in zip(new, lens) for _ in range(n)])
+        tol = 2.0 ** -24 * want.abs() + spread * (
+            2 * (dim + 8) * 2.0 ** -23 * big + 2.0 ** -16 + 2.0 ** -19 * tiles[:, None, None])
+        assert ((got.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_fp32_output_is_the_rounded_output_unrounded(bc, dtype):
+    """Empty rows, masked rows, NaN and rows of nobody as with 16-bit output."""
+    f = make([40, 30], [300, 64], 14, 2, 128, dtype, seed=52)
+    ks = torch.zeros(70, dtype=torch.int32, device="cuda")
+    ks[5], ks[50] = 2 ** 31 - 1, 60
+    f["q"][9, 3, 4] = NAN
+    f["q"] = torch.cat([f["q"], f["q"][:6]])
+    ks = torch.cat([ks, ks[:6]])
+    a = torch.full(f["q"].shape, 7.0, device="cuda")
+    b = a.to(dtype)
+    for out in (a, b):
+        bc.chunk_attention_out(*(f[n] for n in ("q", "k", "v", "pages", "query_start", "lengths")),
+                               out, key_start=ks)
+    assert torch.equal(a.isnan(), b.isnan()) and a[9, 3].isnan().all()
+    assert (a[5] == 0).all() and (b[5] == 0).all() and (a[70:] == 7).all()
+    fin = ~a.isnan()
+    # both within 2^-9 (2^-12) of the weights times |v| < 6 and the output's own rounding
+    eps = torch.finfo(dtype).eps
+    assert ((a - b.float()).abs()[fin] <= eps * (6 + a.abs()[fin])).all()
