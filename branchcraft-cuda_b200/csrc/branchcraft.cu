@@ -1116,7 +1116,9 @@ bool encode_pages_map(CUtensorMap* map, int dtype, const void* base, const bc_sh
 }
 
 bool chunk_shape_ok(const bc_shape* s) {
-  return basic_shape_ok(s) && pool_ok(s->physical_pages) && pool_ok(s->max_pages) &&
+  // (a row's end, rounded up to a key tile, is an int too)
+  return basic_shape_ok(s) && pool_ok(s->physical_pages) &&
+         s->max_pages <= (0x7fffffff - kChTile) / kPageSize &&
          s->batch <= kChMaxBatch && s->query_heads / s->kv_heads <= 128;
 }
 

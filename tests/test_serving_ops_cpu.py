@@ -276,3 +276,14 @@ def test_capi_strides_of_views(monkeypatch):
               torch.zeros(8, 3, 64, dtype=torch.float16).transpose(0, 1)):
         with pytest.raises(ValueError):
             both(cache, cache, x)
+
+
+def test_chunk_refuses_tables_whose_tiles_pass_an_int():
+    """2^31 - 1 keys less a tile: the last key's tile still ends below 2^31."""
+    assert C.chunk_workspace_bytes(shape(max_pages=134217719), 3) > 0
+    assert C.chunk_workspace_bytes(shape(max_pages=134217720), 3) == 0
+    layout = C.KvLayout(2048, 128, 64)
+    opt = C.ChunkOptions(0.125, 0.0, 0, None, None, None)
+    s = shape(max_pages=134217727)
+    assert LIB.bc_chunk_attention(ctypes.byref(s), 3, 0, P, 512, P, P, ctypes.byref(layout), P, P, P,
+                                  ctypes.byref(opt), P, 0, P, 2 ** 40, None) == 1
