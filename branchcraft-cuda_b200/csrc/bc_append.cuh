@@ -49,7 +49,8 @@ struct AppendPlanParams {
   int* positions;            // [max_tokens]
   int* clones;               // [3, batch]: source page, destination page, slots to copy
   int* counts;               // [3]: tokens, clones, status
-  int* scratch;              // [batch + 1]: first pop * 2 + clone flag, then the old free count
+  int* scratch;              // [batch + 1]: first pop * 2 + clone flag (-1: no plan), then the
+                             // old free count
 };
 
 // Shared memory of the planner: the hash table of shared last pages (page,
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(kPlanThreads) append_plan_kernel(const AppendP
     if (!ok) {
       p.query_start[b] = 0;
       p.lengths_out[b] = len;
-      p.scratch[b] = 0;
+      p.scratch[b] = -1;
       continue;
     }
     const AppendSums s = one(b);
@@ -255,18 +256,25 @@ __global__ void __launch_bounds__(kExpandThreads)
   if (int(blockIdx.x) < row_blocks) {
     const int b = blockIdx.x * (kExpandThreads / 32) + (tid >> 5);
     if (b >= p.batch) return;
-    const int n = p.query_start[b + 1] - p.query_start[b], len = p.lengths_out[b] - n;
-    const int have = (len + kPageSize - 1) / kPageSize;  // (<= max_pages_in unless malformed)
-    const int want = (len + n + kPageSize - 1) / kPageSize;
-    const int pop = p.scratch[b] >> 1, clone = p.scratch[b] & 1;
     const int* in = p.pages_in + size_t(b) * p.max_pages_in;
     int* out = p.pages_out + size_t(b) * p.max_pages_out;
     const bool in_place = p.pages_in == p.pages_out;
+    if (p.scratch[b] < 0) {  // no plan: the row as it was, the whole of it at a malformed length
+      const int len = p.lengths_out[b];
+      const int have = len < 0 || len > p.max_pages_in * kPageSize ? p.max_pages_in
+                                                                   : (len + kPageSize - 1) / kPageSize;
+      for (int c = lane; c < p.max_pages_out && !in_place; c += 32) out[c] = c < have ? in[c] : -1;
+      return;
+    }
+    const int n = p.query_start[b + 1] - p.query_start[b], len = p.lengths_out[b] - n;
+    const int have = (len + kPageSize - 1) / kPageSize;  // (<= max_pages_in)
+    const int want = (len + n + kPageSize - 1) / kPageSize;
+    const int pop = p.scratch[b] >> 1, clone = p.scratch[b] & 1;
     const int first = in_place ? have - clone : 0, end = in_place ? want : p.max_pages_out;
     for (int c = first + lane; c < end; c += 32) {
       int page = -1;
       if (c < have - clone || (c < have && !clone)) {
-        page = c < p.max_pages_in ? in[c] : -1;
+        page = in[c];
       } else if (c < want) {
         if (c < have) atomicSub(&p.refcount[in[c]], 1);  // the cloned page's reference
         page = p.free_stack_in[top - (pop + c - (have - clone))];

@@ -322,3 +322,20 @@ def test_plan_and_rows_in_a_graph(bc):
         assert (ck.view(-1, 2, 64)[slot_map.long()] == step + 1).all()
     assert pages.tolist() == pool.page_table(reqs, 6)
     S.assert_pool(pool, *state)
+
+
+@pytest.mark.parametrize("length", [-1, -2 ** 31, 145, 2 ** 31 - 1, 2 ** 31 - 14, 100])
+def test_failed_plans_keep_rows(bc, length):
+    """New tables after a plan that failed hold the rows as they were, at malformed lengths
+    too (there the whole row)."""
+    pages = torch.arange(27, dtype=torch.int32, device="cuda").view(3, 9).contiguous()
+    lengths = ints([40, length, 144])
+    state = ints([1] * 40), ints(list(range(40))), ints([40])
+    for new, width in ((ints([1, 0, 1]), 9), (ints([1, 1, -1]), 12), (ints([0, 0, 200]), 9)):
+        out = bc.append_plan(pages, lengths, new, *state, 300, width)
+        assert out[9][2].item() != 0 and torch.equal(out[1], lengths)
+        want = torch.full((3, width), -1, dtype=torch.int32, device="cuda")
+        for b, x in enumerate((40, length, 144)):
+            n = (x + 15) // 16 if 0 <= x <= 144 else 9
+            want[b, :n] = pages[b, :n]
+        assert torch.equal(out[0], want)
