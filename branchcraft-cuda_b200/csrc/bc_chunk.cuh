@@ -455,9 +455,9 @@ __global__ void __launch_bounds__(kChThreads, 1)
       // ------------------------------------------- scheduler and V producer
       // This block's share: from its own cut (found by lanes 0-15) up to the next
       // block's (lanes 16-31). Cuts inside an item fall on multiples of `grain`
-      // tiles from its start (a thirty-second of a share, at least 2: eighths of a
-      // share left blocks a quarter apart, single tiles cost the prompts 2 %) or on
-      // its ends; an item of no more than kChWhole tiles has no cut.
+      // tiles from its start (a thirty-second of a share, at least 2, which bounds what
+      // rounding adds to a block) or on its ends; an item of no more than kChWhole
+      // tiles has no cut.
       const int half = lane >> 4, hl = lane & 15;
       const int per_lane = (p.batch + 15) / 16;
       const int sb0 = min(p.batch, hl * per_lane), sb1 = min(p.batch, sb0 + per_lane);
@@ -959,23 +959,40 @@ __global__ void __launch_bounds__(kChThreads, 1)
           }
           mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
         }
-        if constexpr (MOD == 0) mx *= p.scale_log2;  // -inf stays -inf
+        float mul = 1.f;  // of a score, in the exponent
+        if constexpr (MOD == 0) {
+          mul = p.scale_log2;
+          mx *= mul;  // -inf stays -inf
+          // The exponent's multiply-add does not round its product, the maximum does: a
+          // difference of powers of 2 once scores pass 2^24, of their sixteenths here.
+          // Such rows' scores are rounded first, so that none passes the maximum.
+          if (fabsf(mx) > 1048576.f && mx != kNegInf) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                s[c][e] = __float_as_uint(__fmul_rn(__uint_as_float(s[c][e]), mul));
+            mul = 1.f;
+          }
+          __syncwarp();
+        }
         // P of the last tile has been read, and O holds its product.
         ok = p_taken() && zero_pads(j, k0);
         if (!ok) break;
         ++sc;
         tc_fence_after();
-        // Lazy maximum: the reference moves only when a row's maximum grows by
-        // more than 2^8, with probabilities up to 2^8 until then. FP16 ones (and with
-        // them l and O) are held times 2^7, up to 2^15: without it those below 2^-25 of
-        // the largest were rounded to 0, and of tens of thousands of keys such ones can
-        // make a thousandth of the output.
+        // Lazy maximum: the reference moves only when it falls 2^kLag behind a row's
+        // maximum, which probabilities may reach until then. For FP16 it is set 2^7 below
+        // the maximum: otherwise those below 2^-25 of the largest were rounded to 0, and
+        // of tens of thousands of keys such ones can make a thousandth of the output.
+        constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f, kLag = kLift + 8.f;
         float alpha = 1.f;
         bool rescale = false;
-        if (mx > m_ref + 8.f) {
-          alpha = fast_exp2(m_ref - mx);
+        if (mx - m_ref > kLag) {  // (no sum of them: past 2^24 that would round up)
+          const float next = mx - kLift;
+          alpha = fast_exp2(m_ref - next);
           rescale = m_ref != kNegInf;
-          m_ref = mx;
+          m_ref = next;
           l_sum *= alpha;
         }
         // O moves to the new reference (rare; eight columns at a time, the scores
@@ -993,8 +1010,7 @@ __global__ void __launch_bounds__(kChThreads, 1)
           }
           tmem_st_wait();
         }
-        constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
-        const float mb = m_ref == kNegInf ? 0.f : kLift - m_ref;
+        const float mb = m_ref == kNegInf ? 0.f : -m_ref;
         float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -1003,9 +1019,9 @@ __global__ void __launch_bounds__(kChThreads, 1)
           for (int e = 0; e < 32; e += 4) {
             float x0, x1, x2, x3;
             fma_pair(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]),
-                     MOD ? 1.f : p.scale_log2, mb, x0, x1);
+                     mul, mb, x0, x1);
             fma_pair(__uint_as_float(s[c][e + 2]), __uint_as_float(s[c][e + 3]),
-                     MOD ? 1.f : p.scale_log2, mb, x2, x3);
+                     mul, mb, x2, x3);
             x0 = fast_exp2(x0);
             x1 = fast_exp2(x1);
             x2 = fast_exp2(x2);

@@ -293,3 +293,39 @@ def test_fp32_output_is_the_rounded_output_unrounded(bc, dtype):
     # both within 2^-9 (2^-12) of the weights times |v| < 6 and the output's own rounding
     eps = torch.finfo(dtype).eps
     assert ((a - b.float()).abs()[fin] <= eps * (6 + a.abs()[fin])).all()
+
+
+# ------------------------------------------------------------- very large scores
+
+
+@pytest.mark.parametrize("dtype,dim,size", [
+    (F16, 128, 200.0), (F16, 64, 3000.0), (F16, 128, 60000.0), (BF16, 128, 200.0),
+    (BF16, 64, 3e9), (BF16, 128, 1e18)])
+@pytest.mark.parametrize("new,length", [(1, 17), (40, 300), (1, 20000), (150, 3000)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_any_finite_size(bc, new, length, sign, dtype, dim, size):
+    """Scores from 10^5 to 10^38, whose last place is many powers of e. All equal: the mean of
+    the seen values. One key a 64th above the others: that key's value alone."""
+    f = make([new], [length], 4, 2, dim, dtype, seed=61)
+    f["q"].fill_(sign * size)
+    f["k"].fill_(size)
+    ids = f["pages"][0, :(length + 15) // 16].long()
+    v = f["v"][ids].flatten(0, 1)[:length].cpu().double().repeat_interleave(2, 1)
+    at = length - new + torch.arange(new)
+    got = bc.chunk_attention(**f).cpu().double()
+    want = v.cumsum(0)[at] / (at + 1.0)[:, None, None]
+    spread = v.abs().cumsum(0)[at] / (at + 1.0)[:, None, None]
+    # equal weights, each rounded to 16 bits; the sums' FP32 additions (sixteen a tile at most,
+    # 2^-23 each) and the output's rounding
+    u = torch.finfo(dtype).eps / 2
+    tol = u * want.abs() + spread * (1 + u) * (u + 2.0 ** -16 + 2.0 ** -19 * ((length + 127) // 128))
+    assert ((got - want).abs() <= tol).all()
+    first = length // 2
+    f["k"][ids[first // 16], first % 16] *= 1 + sign / 64
+    seen = at >= first
+    got = bc.chunk_attention(**f).cpu().double()
+    # Its weight need not be 1: up to 2^20 (in log2 units) the exponent is the unrounded
+    # product less its rounded value, up to 2^-5 apart, so the weight 2^(2^-5) at most. That
+    # is rounded to 16 bits (u) in the product and not in the sum; then the output's u.
+    alone = v[first].expand(int(seen.sum()), -1, -1)
+    assert ((got[seen] - alone).abs() <= 2 * u * (1 + u) * alone.abs()).all()
