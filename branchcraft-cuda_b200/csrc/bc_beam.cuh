@@ -5,6 +5,8 @@
 
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "bc_attn.cuh"
 
 namespace bc {
@@ -110,6 +112,19 @@ __device__ __forceinline__ double beam_value64(unsigned long long u) {
   return __longlong_as_double(u >> 63 ? u & ~(1ull << 63) : ~u);
 }
 
+// The 16 bytes from byte `by` (below 16) of 32 on.
+__device__ __forceinline__ uint4 beam_shift(uint4 lo, uint4 hi, unsigned by) {
+  const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+  uint32_t a[6], b[5];
+#pragma unroll
+  for (int i = 0; i < 6; ++i) a[i] = by & 8u ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) b[i] = by & 4u ? a[i + 1] : a[i];
+  const unsigned bits = (by & 3u) * 8u;
+  return make_uint4(__funnelshift_r(b[0], b[1], bits), __funnelshift_r(b[1], b[2], bits),
+                    __funnelshift_r(b[2], b[3], bits), __funnelshift_r(b[3], b[4], bits));
+}
+
 struct BeamSelectParams {
   int batch, beams, vocab, k;
   int segments, segment;  // blocks of a row, their steps' logits (a multiple of the step)
@@ -205,23 +220,26 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const Bea
   grid_dependency_wait();
   const int row = blockIdx.x / p.segments, seg = blockIdx.x % p.segments;
   const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
-  // Places count from the 16-byte boundary at or before the row: place = token + mis.
-  const int mis = int((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const T* x0 = x - mis;
-  const int w0 = seg * p.segment, w1 = min(w0 + p.segment, p.vocab + mis);
+  // Threads take tokens by their numbers wherever the row lies, so that rows alike are
+  // summed alike, to the last bit: pairs of such beams are equal, and ordered by their
+  // index. A row off the 16-byte boundaries puts its vectors together from the two
+  // aligned ones that hold them (each of which holds a logit of the row).
+  const unsigned mis = unsigned(reinterpret_cast<uintptr_t>(x) & 15);  // bytes
+  const uint4* lines = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x) - mis);
+  const int w0 = seg * p.segment, w1 = min(w0 + p.segment, p.vocab);
   const float score = p.scores[row];
   auto load = [&](int w, uint32_t (&raw)[16]) {
 #pragma unroll
     for (int j = 0; j < kBeamLoads; ++j) {
       const int at = w + (j * kBeamThreads + tid) * VEC;
       uint4 v;
-      if (at >= mis && at + VEC <= p.vocab + mis) {
-        v = __ldcs(reinterpret_cast<const uint4*>(x0 + at));
-      } else {  // a vector across the row's ends: its own logits alone
+      if (at + VEC <= p.vocab) {
+        v = __ldcs(lines + at / VEC);
+        if (mis) v = beam_shift(v, __ldcs(lines + at / VEC + 1), mis);
+      } else {  // a vector across the row's end: its own logits alone
         T e[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          e[i] = at + i >= mis && at + i < p.vocab + mis ? x0[at + i] : T(-INFINITY);
+        for (int i = 0; i < VEC; ++i) e[i] = at + i < p.vocab ? x[at + i] : T(-INFINITY);
         v = *reinterpret_cast<const uint4*>(e);
       }
       raw[4 * j] = v.x;
@@ -230,16 +248,41 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const Bea
       raw[4 * j + 3] = v.w;
     }
   };
+  // The same for the stream, where the words' place is settled once a step.
+  auto words = [&](auto skip, int w, uint32_t (&raw)[16]) {
+    constexpr int S = decltype(skip)::value;  // whole words of `mis`
+    const unsigned bits = (mis & 3u) * 8u;
+#pragma unroll
+    for (int j = 0; j < kBeamLoads; ++j) {
+      const int at = w + (j * kBeamThreads + tid) * VEC;
+      const uint4 lo = __ldcs(lines + at / VEC), hi = __ldcs(lines + at / VEC + 1);
+      const uint32_t v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        raw[4 * j + i] = sizeof(T) == 4 ? v[i + S] : __funnelshift_r(v[i + S], v[i + S + 1], bits);
+    }
+  };
+  auto fetch = [&](int w, uint32_t (&raw)[16]) {
+    if (mis == 0 || w + TILE > p.vocab) {
+      load(w, raw);
+    } else {
+      switch (mis >> 2) {
+        case 0: words(std::integral_constant<int, 0>{}, w, raw); break;
+        case 1: words(std::integral_constant<int, 1>{}, w, raw); break;
+        case 2: words(std::integral_constant<int, 2>{}, w, raw); break;
+        default: words(std::integral_constant<int, 3>{}, w, raw);
+      }
+    }
+  };
   uint32_t raw[16], next[16];
-  if (w0 < w1) load(w0, raw);
+  if (w0 < w1) fetch(w0, raw);
   // A beam that is out: all its pairs score -inf, so its first tokens are its best,
   // whatever their logits. (Looked at with the first logits on their way: beside
   // them, the score costs no wait of its own.)
   if (beam_score(score) == -INFINITY) {
-    const int first = max(w0 - mis, 0);
     for (int i = tid; i < p.k; i += kBeamThreads)
       p.keys[size_t(blockIdx.x) * p.k + i] =
-          first + i < w1 - mis ? beam_key(-INFINITY, unsigned(first + i)) : 0ull;
+          w0 + i < w1 ? beam_key(-INFINITY, unsigned(w0 + i)) : 0ull;
     if (tid == 0) {
       p.seg_max[blockIdx.x] = -INFINITY;
       p.seg_sum[blockIdx.x] = 0.0;
@@ -270,7 +313,7 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const Bea
   double sum = 0.0;
   int top = w0;  // the first step with the largest logit
   for (int w = w0, i = 0; w < w1; w += TILE, ++i) {
-    if (w + TILE < w1) load(w + TILE, next);
+    if (w + TILE < w1) fetch(w + TILE, next);
     const float mx = clean();
     if (i < kBeamSteps) step_max[i * kBeamThreads] = mx;
     if (mx > m) {
@@ -297,8 +340,8 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const Bea
     clean();
     for (uint32_t bits = at_or_above(m); bits; bits &= bits - 1) {
       const int at = place(w, __ffs(bits) - 1);
-      if (at >= mis && at < w1) {
-        best = beam_key(m, unsigned(at - mis));
+      if (at < w1) {
+        best = beam_key(m, unsigned(at));
         break;
       }
     }
@@ -328,9 +371,9 @@ __global__ void __launch_bounds__(kBeamThreads, 4) beam_segment_kernel(const Bea
     if (clean() >= bound)
       for (uint32_t bits = at_or_above(bound) & of; bits; bits &= bits - 1) {
         const int at = place(w, __ffs(bits) - 1);
-        if (at < mis || at >= w1) continue;
+        if (at >= w1) continue;
         // (few: read again, rather than picked out of the registers)
-        const unsigned long long key = beam_key(beam_one(x0[at]), unsigned(at - mis));
+        const unsigned long long key = beam_key(beam_one(x[at]), unsigned(at));
         if (key < tau) continue;
         const int i = atomicAdd(&s_n, 1);
         if (i < room) beam_cand[i] = key;
@@ -449,9 +492,8 @@ __global__ void __launch_bounds__(kBeamMergeThreads) beam_merge_kernel(const Bea
   };
   for (int l = tid; l < lists; l += kBeamMergeThreads) {
     const unsigned long long key = keys[size_t(l) * p.k];
-    // (a segment past a row's end has an empty list: behind all others)
-    head_v[l] = key == 0 ? 0ull : value(l, key);
-    head_i[l] = key == 0 ? 0xffffffffu - unsigned(l) : index(l, key);
+    head_v[l] = value(l, key);  // (every segment has a logit: no list is empty)
+    head_i[l] = index(l, key);
   }
   __syncthreads();
   for (int l = tid; l < lists; l += kBeamMergeThreads) {  // the k-th best head

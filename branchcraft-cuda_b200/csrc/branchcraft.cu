@@ -1214,7 +1214,7 @@ struct BeamPlan {
   int segments, segment;
   BeamPlan(int rows, int vocab, int type_bytes, int dev) {
     const int tile = beam_tile(type_bytes);
-    const int steps = (vocab + 15 + tile - 1) / tile;  // (from a 16-byte boundary on)
+    const int steps = (vocab + tile - 1) / tile;
     const long long slots = 4ll * (dev < 0 ? 148 : sm_count(dev));
     long long least = -1;
     int per = steps;
@@ -1227,7 +1227,7 @@ struct BeamPlan {
       }
     }
     segment = per * tile;
-    segments = (vocab + 15 + segment - 1) / segment;
+    segments = (vocab + segment - 1) / segment;
   }
 };
 

@@ -283,3 +283,15 @@ def test_select_beams_that_are_out(bc, dtype, out):
             check_select(bc, x, scores, k)
             scores[1, dead] = out
             check_select(bc, x, scores, min(k, allowed + 1))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [5, 1001, 8192, 32001, 50257, 131071, 200003])
+def test_select_beams_alike(bc, dtype, vocab):
+    """Beams with the same logits and scores (a first step): equal pairs by the lowest index,
+    however the beams' rows lie to the memory's 16-byte pieces."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    for beams, k in ((4, 8), (8, 16), (3, 5)):
+        x = (torch.randn(3, 1, vocab, generator=g, device="cuda") * 3).to(dtype)
+        x = x.expand(3, beams, vocab).contiguous()
+        check_select(bc, x, torch.zeros(3, beams, device="cuda"), k)
